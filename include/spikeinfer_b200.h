@@ -704,6 +704,118 @@ typedef struct spk_experts_args {
 } spk_experts_args;
 int spk_experts(const spk_experts_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * 8-bit rows and products.  An e4m3 matrix [rows, columns] has rows that start on 16-byte boundaries (row stride a multiple of 16, what lies
+ * behind the columns is not read); activations carry one 32-bit scale for every row and 128 columns, weights one for every block of
+ * 128 x 128.  A value stands for value * scale.
+ * ------------------------------------------------------------------------- */
+enum {
+    SPK_ACT_NONE = 0,
+    SPK_ACT_GELU_TANH = 1,
+    SPK_ACT_SILU_GATE = 2   /* silu(z[t, c]) * z[t, width + c] */
+};
+
+/* One layer boundary with an 8-bit output: y = x + delta + sum_j pair_weights[t, j] * pairs[pair_slots[t, j]] (delta, pairs may be NULL; a negative
+ * slot counts as zero), rounded to x_dtype; x_out <- y (may alias x, may be NULL); v = y / rms(y) * w; out <- v (may be NULL); q, scales <- v in
+ * 8 bits: scales[b * scale_stride + t] = max(largest |v| of columns 128 b .. 128 b + 127, 2^-100) / 448, q = v / scale to the nearest, at most 448.
+ * NaN stays NaN and is not the largest; an infinity counts as the largest finite value.  x_dtype SPK_BF16: delta is SPK_BF16 too. */
+typedef struct spk_rms_residual_fp8_args {
+    const void* x;              /* [n, width] */
+    const void* delta;          /* [n, width] */
+    void* x_out;
+    const float* w;             /* [width] */
+    const float* pairs;         /* [pair_rows, width] */
+    const int32_t* pair_slots;  /* [n, pair_top] */
+    const float* pair_weights;  /* [n, pair_top] */
+    void* out;                  /* [n, width] in out_dtype */
+    void* q;                    /* e4m3 [n, width], row stride q_stride bytes; 16-byte aligned */
+    float* scales;
+    int64_t pair_rows;
+    int64_t n;
+    int64_t width;
+    int64_t q_stride;
+    int64_t scale_stride;
+    int32_t pair_top;
+    int32_t x_dtype;
+    int32_t delta_dtype;
+    int32_t out_dtype;
+    float eps;
+    int32_t _pad;
+    uint32_t* status;
+} spk_rms_residual_fp8_args;
+int spk_rms_residual_fp8(const spk_rms_residual_fp8_args* args, void* stream);
+
+/* The same 8-bit form of act(z), z [n, width] (SPK_ACT_SILU_GATE: [n, 2 width]) with row stride z_stride elements. */
+typedef struct spk_quantize_fp8_args {
+    const void* z;
+    void* q;
+    float* scales;
+    int64_t z_stride;
+    int64_t q_stride;
+    int64_t scale_stride;
+    int64_t n;
+    int64_t width;
+    int32_t act;
+    int32_t dtype;
+} spk_quantize_fp8_args;
+int spk_quantize_fp8(const spk_quantize_fp8_args* args, void* stream);
+
+/* out[t, f] = sum_b x_scales[b * x_scale_stride + t] * w_scales[(f / 128) * w_scale_stride + b] * (sum of x[t, c] w[f, c] over columns c of block b), sums
+ * in 32 bits, out in out_dtype (SPK_F32 or SPK_BF16) with row stride out_stride elements.  x [n, k] and w [features, k] in e4m3, 16-byte aligned, row
+ * strides x_stride and w_stride bytes.  The result does not depend on timing. */
+typedef struct spk_linear_fp8_args {
+    const void* x;
+    const void* w;
+    const float* x_scales;
+    const float* w_scales;
+    void* out;
+    int64_t x_stride;
+    int64_t w_stride;
+    int64_t x_scale_stride;
+    int64_t w_scale_stride;
+    int64_t out_stride;
+    int64_t n;
+    int64_t k;
+    int64_t features;
+    int32_t out_dtype;
+    int32_t _pad;
+    uint32_t* status;
+} spk_linear_fp8_args;
+int spk_linear_fp8(const spk_linear_fp8_args* args, void* stream);
+
+/* Experts chosen by scores.  Per token: s = softmax(logits) or 1 / (1 + exp(-logits)), c = s + bias (bias may be NULL).  groups > 1: the experts are cut into
+ * `groups` equal runs, a group counts the sum of its best two c, and only the best top_groups groups stay.  ids [n, top] <- the best c in falling order,
+ * equal ones by index; weights [n, top] <- s of these, divided by their sum with renormalize (0 where that is 0), times scale.  An expert whose logit or
+ * c is NaN or -infinity is never chosen (+infinity counts as the largest finite 32-bit value); choices that are left over, and all of a token whose
+ * active is not 1, get id -1, weight 0 and slot -1.  Comparisons have the outcome of 64-bit arithmetic.
+ * slots [n, top] <- row of the (token, choice) pair in the matrix sorted by expert, pairs in their order inside a segment; segs [experts, 2] <- first row
+ * and rows of every expert; first rows are multiples of eight (spk_expert_rows, spk_experts).
+ * experts <= 1024, top <= 32; workspace of spk_route_scores_workspace_bytes(n, experts) bytes. */
+enum {
+    SPK_SCORE_SOFTMAX = 0,
+    SPK_SCORE_SIGMOID = 1
+};
+typedef struct spk_route_scores_args {
+    const void* logits;         /* [n, experts], row stride logits_stride elements */
+    const float* bias;          /* [experts] or NULL */
+    const int32_t* active;      /* [n] or NULL */
+    int32_t* ids;
+    float* weights;
+    int32_t* slots;
+    int32_t* segs;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t logits_stride;
+    int64_t n;
+    int32_t dtype;              /* SPK_F32 or SPK_BF16 */
+    int32_t experts, top, groups, top_groups;
+    int32_t score;
+    int32_t renormalize;
+    float scale;
+} spk_route_scores_args;
+int64_t spk_route_scores_workspace_bytes(int64_t n, int experts);
+int spk_route_scores(const spk_route_scores_args* args, void* stream);
+
 /* Cache row of the latent attention: `rank` latent channels, then (from channel rank_pad) rot_dim rotated ones.  A pool is
  * [num_blocks][block_size][rank_pad + rot_pad]; tiled (csrc/spk_latent.cuh), or plain with rank_pad == rank, rot_pad == rot_dim.
  *

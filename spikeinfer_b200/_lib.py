@@ -27,6 +27,9 @@ STATUS_ROW_BUSY = 1 << 6
 STATUS_DEVICE_WAIT_EXPIRED = 1 << 7
 STATUS_BAD_TOKEN = 1 << 8
 
+ACT_NONE, ACT_GELU_TANH, ACT_SILU_GATE = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
 ROW_FREE, ROW_DECODING, ROW_HELD = 0, 1, 2
 
 MAX_LIF_SITES = 4
@@ -207,6 +210,32 @@ class RowsLinearArgs(Structure):
     _fields_ = _fields("p x w out; l ld_x ld_out n k features; i out_dtype overlap")
 
 
+class RmsResidualFp8Args(Structure):
+    """Mirror of ``spk_rms_residual_fp8_args``."""
+
+    _fields_ = _fields("p x delta x_out w pairs pair_slots pair_weights out q scales; l pair_rows n width q_stride scale_stride; "
+                       "i pair_top x_dtype delta_dtype out_dtype; f eps; i _pad; p status")
+
+
+class QuantizeFp8Args(Structure):
+    """Mirror of ``spk_quantize_fp8_args``."""
+
+    _fields_ = _fields("p z q scales; l z_stride q_stride scale_stride n width; i act dtype")
+
+
+class LinearFp8Args(Structure):
+    """Mirror of ``spk_linear_fp8_args``."""
+
+    _fields_ = _fields("p x w x_scales w_scales out; l x_stride w_stride x_scale_stride w_scale_stride out_stride n k features; i out_dtype _pad; p status")
+
+
+class RouteScoresArgs(Structure):
+    """Mirror of ``spk_route_scores_args``."""
+
+    _fields_ = _fields("p logits bias active ids weights slots segs workspace; l workspace_bytes logits_stride n; "
+                       "i dtype experts top groups top_groups score renormalize; f scale")
+
+
 class SpikePortion(Structure):
     """Mirror of ``spk_spike_portion``."""
 
@@ -294,6 +323,11 @@ SIGNATURES = {
     "spk_gated_norm": (c_int, [POINTER(GatedNormArgs), c_void_p]),
     "spk_rms_residual": (c_int, [POINTER(RmsResidualArgs), c_void_p]),
     "spk_rows_linear": (c_int, [POINTER(RowsLinearArgs), c_void_p]),
+    "spk_rms_residual_fp8": (c_int, [POINTER(RmsResidualFp8Args), c_void_p]),
+    "spk_quantize_fp8": (c_int, [POINTER(QuantizeFp8Args), c_void_p]),
+    "spk_linear_fp8": (c_int, [POINTER(LinearFp8Args), c_void_p]),
+    "spk_route_scores_workspace_bytes": (c_int64, [c_int64, c_int]),
+    "spk_route_scores": (c_int, [POINTER(RouteScoresArgs), c_void_p]),
     "spk_gelu_tanh": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "spk_expert_route": (c_int, [POINTER(ExpertRouteArgs), c_void_p]),
     "spk_expert_rows": (c_int64, [c_int64, c_int, c_int]),

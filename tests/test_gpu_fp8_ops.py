@@ -1,0 +1,293 @@
+"""GPU: the 8-bit operators and the experts chosen by scores, each alone, against plain forms in float64.
+
+Tolerances count roundings: u = 2^-24 is half a step of fp32, 2^-8 of bf16, 2^-4 of e4m3."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import fp8_oracle as fo
+from spikeinfer_b200 import _lib
+from spikeinfer_b200.kernels import fp8 as k8
+from spikeinfer_b200.kernels import routing as kr
+
+pytestmark = pytest.mark.gpu
+F32, BF, FP8 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+U = 2.0 ** -24
+HALF = {F32: U, BF: 2.0 ** -8}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def holds8(q, scales, v, rel):
+    """q and scales are the 8-bit form of v, known to a relative error of `rel`."""
+    v = v.double().cpu()
+    width = v.shape[1]
+    want = fo.block_scales(v)
+    assert q.dtype == FP8 and q.shape == v.shape and scales.shape == want.shape and scales.dtype == F32
+    assert ((scales.double().cpu() - want).abs() <= (rel + 2 * U) * want).all()
+    s = fo.spread(scales.cpu(), width)
+    got = q.cpu().double()
+    off = (got * s - v).abs()
+    # half a step of the quotient, whose own error (that of v, two roundings) can reach over the middle between two values
+    assert (off <= (0.5 * fo.e4m3_step(v / s) + (rel + 4 * U) * 512) * s).all()
+    assert ((off <= 0.5 * fo.e4m3_step(v / s) * s * (1 + 64 * U) + (rel + 4 * U) * v.abs())).all()
+    for b in range(want.shape[0]):  # the largest of a block is 448
+        there = want[b] > fo.LEAST / 448
+        assert (got[:, 128 * b: 128 * b + 128].abs().amax(1)[there] == 448).all()
+
+
+# ---- boundary --------------------------------------------------------------------------------------------------------
+# v = y * rms * w: a sum of squares over at most 21 roundings a term, its root half of that, and five more: 16 u
+NORM = 16 * U
+
+
+@pytest.mark.parametrize("stream,delta_dtype", [(F32, F32), (F32, BF), (F32, None), (BF, BF), (BF, None)])
+@pytest.mark.parametrize("n,width,top", [(1, 1, 0), (1, 45, 1), (37, 88, 3), (5, 129, 0), (3, 896, 0), (2, 1022, 2), (64, 3584, 2), (7, 1028, 6), (3, 9001, 2),
+                                         (2, 32768, 1), (700, 256, 0), (601, 1030, 2)])
+def test_boundary(dev, n, width, top, stream, delta_dtype):
+    g = gen(n * 7 + width)
+    rnd = lambda *s: torch.randn(*s, generator=g)
+    x, w, eps = rnd(n, width).to(stream), 1 + 0.3 * rnd(width), 1e-5
+    delta = None if delta_dtype is None else rnd(n, width).to(delta_dtype)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    args, more = {}, 0.0
+    if top:
+        rows = n * top + 5
+        slots = torch.randperm(rows, generator=g)[: n * top].view(n, top).to(torch.int32)
+        slots[torch.rand(n, top, generator=g) < 0.2] = -1
+        pairs, weights = rnd(rows, width), torch.rand(n, top, generator=g)
+        pairs[[r for r in range(rows) if r not in set(slots.flatten().tolist())]] = float("nan")
+        args = dict(pairs=pairs, slots=slots, weights=weights)
+        more = fo.boundary(torch.zeros(n, width), None, pairs.abs(), slots, weights)
+    y = fo.boundary(x, delta, **args)
+    size = x.double().abs() + (0 if delta is None else delta.double().abs()) + more
+    d = lambda t: None if t is None else t.to(dev)
+    on = dict(pairs=d(args["pairs"]), pair_slots=d(args["slots"]), pair_weights=d(args["weights"])) if top else {}
+    x_out = torch.full((n, width), 7.0, dtype=stream, device=dev)
+    for out_dtype in (BF, F32):
+        out = torch.full((n, width), 7.0, dtype=out_dtype, device=dev)
+        xd = d(x)
+        q, scales = k8.rms_residual_fp8(xd, d(w), eps=eps, delta=d(delta), x_out=x_out, out=out, status=status, **on)
+        assert torch.equal(xd, d(x))
+        assert ((x_out.double().cpu() - y).abs() <= (top + 2) * U * size + (HALF[BF] * (y.abs() + 2 * U * size) if stream == BF else 0)).all()
+        v = fo.rms_norm(x_out.cpu(), w, eps)  # of what is stored
+        assert ((out.double().cpu() - v).abs() <= (NORM + HALF[out_dtype]) * (1 + 2 * U) * v.abs()).all()
+        holds8(q, scales, v, NORM)
+    # in place, without the plain output: the same bits
+    xd = d(x)
+    q2, s2 = k8.rms_residual_fp8(xd, d(w), eps=eps, delta=d(delta), x_out=xd, status=status, **on)
+    assert torch.equal(xd, x_out) and torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, scales)
+    # and without keeping the sum
+    q2, s2 = k8.rms_residual_fp8(d(x), d(w), eps=eps, delta=d(delta), status=status, **on)
+    assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, scales)
+    assert int(status.item()) == 0
+
+
+def test_boundary_reports_slots_that_do_not_exist(dev):
+    x, w = torch.randn(4, 64, device=dev), torch.ones(64, device=dev)
+    pairs, weights = torch.randn(8, 64, device=dev), torch.ones(4, 2, device=dev)
+    slots = torch.tensor([[0, 1], [8, 2], [-1, -5], [3, 2 ** 30]], dtype=torch.int32, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    x_out = torch.empty_like(x)
+    k8.rms_residual_fp8(x, w, eps=1e-5, x_out=x_out, pairs=pairs, pair_slots=slots, pair_weights=weights, status=status)
+    assert int(status.item()) == _lib.STATUS_BAD_SLOT
+    want = fo.boundary(x.cpu(), None, pairs.cpu(), slots.cpu(), weights.cpu())
+    assert ((x_out.double().cpu() - want).abs() <= 4 * U * 10).all()
+
+
+def test_values_that_are_not_finite_and_blocks_of_nothing(dev):
+    z = torch.zeros(6, 300)
+    z[0, 3], z[0, 200] = float("nan"), 2.0
+    z[1, 5], z[1, 6], z[1, 140] = float("inf"), 1.0, -float("inf")
+    z[2, :128] = float("nan")
+    z[3, 17] = 1e-35
+    z[4, 0], z[4, 1] = 3e38, 1e30
+    z[5, 299] = -5.0
+    q, s = k8.quantize_fp8(z.to(dev))
+    q, s = q.double().cpu(), s.double().cpu()
+    top = torch.finfo(torch.float32).max
+    assert q[0, 3].isnan() and int(q.isnan().sum()) == 129
+    assert abs(float(s[0, 1]) / (top / 448) - 1) < 4 * U and q[1, 5] == 448 and q[1, 6] == 0 and q[1, 140] == -448
+    assert q[2, :128].isnan().all() and (s[0, [0, 2, 3, 5]] == torch.tensor(2.0 ** -100 / 448, dtype=F32).double()).all()
+    assert q[4, 0] == 448 and q[4, 1] == 0 and q[5, 299] == -448 and q[0, 200] == 448
+    assert torch.isfinite(s).all() and (s > 0).all()
+
+
+# ---- activations -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("act", ["none", "gelu_tanh", "silu_gate"])
+@pytest.mark.parametrize("n,width,pad", [(1, 1, 0), (3, 45, 3), (37, 4864, 0), (130, 896, 8), (5, 1021, 1), (2, 18944, 0), (65, 128, 0), (33, 130, 2)])
+def test_quantize(dev, n, width, pad, act, dtype):
+    z = 3 * torch.randn(n, width * (2 if act == "silu_gate" else 1), generator=gen(n + width)).to(dtype)
+    big = torch.full((n, z.shape[1] + pad), float("nan"), dtype=dtype, device=dev)
+    view = big[:, pad // 2: pad // 2 + z.shape[1]]
+    view.copy_(z)
+    q, scales = k8.quantize_fp8(view, act)
+    v = fo.activation(z, act)
+    # the exponential and what stands in its exponent (|z| <= 18: its three roundings and the function's 2 ulp at up to 200), the quotient and the product
+    rel = 0.0 if act == "none" else (1300 if act == "gelu_tanh" else 64) * U
+    want = fo.block_scales(v)
+    assert ((scales.double().cpu() - want).abs() <= (rel + 2 * U) * want).all()
+    s = fo.spread(scales.cpu(), width)
+    off = (q.double().cpu() * s - v).abs()
+    # far tails of the gelu are off by more; under 1e-4 of its block's largest a value is under 0.0448 of the scale, so under 2^-4, where half a step is 2^-9 or less
+    keep = v.abs() > 1e-4 * 448 * s
+    assert (off <= 0.5 * fo.e4m3_step(v / s) * s * (1 + 64 * U) + (rel + 4 * U) * v.abs())[keep | (act == "none")].all()
+    assert (off <= 1.01 * 2.0 ** -9 * s)[~keep].all()
+
+
+# ---- products --------------------------------------------------------------------------------------------------------
+def operands(n, k, f, dev, seed, pad=0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    x, w = (torch.full((r, -(-k // 16) * 16 + 16 * pad), float("nan"), device=dev).to(FP8)[:, :k] for r in (n, f))  # NaN behind the columns
+    x.copy_((150 * torch.randn(n, k, generator=g, device=dev)).clamp(-448, 448))
+    w.copy_((150 * torch.randn(f, k, generator=g, device=dev)).clamp(-448, 448))
+    blocks = -(-k // 128)
+    sx = torch.exp2(4 * torch.randn(blocks, n + pad, generator=g, device=dev))[:, :n]  # a row's blocks differ by a lot: a scale at the wrong place shows
+    sw = torch.exp2(2 * torch.randn(-(-f // 128), blocks, generator=g, device=dev))
+    return x, sx, w, sw
+
+
+def check_linear(out, x, sx, w, sw):
+    want, size = fo.linear(x.cpu(), sx.cpu(), w.cpu(), sw.cpu())
+    # products are exact.  A tensor-core step adds 32 of them and the sum so far, each cut to 23 bits or more of the largest: 4 steps of 33 terms within
+    # 2^-23 of the block's magnitudes; then a product of scales, a product with it and a sum per block
+    tol = (132 * 2.0 ** -23 + (3 + -(-x.shape[1] // 128)) * U) * size
+    off = (out.double().cpu() - want).abs()
+    assert (off <= tol + HALF[out.dtype] * (want.abs() + tol)).all(), float((off / size.clamp(min=1e-300)).max())
+
+
+SIZES = [(1, 16, 1), (1, 45, 7), (1, 128, 128), (3, 129, 130), (1, 896, 4864), (16, 256, 300), (17, 384, 129), (31, 1000, 257), (33, 640, 200), (64, 3584, 896),
+         (65, 128, 512), (100, 4864, 130), (128, 512, 128), (129, 1021, 255), (200, 2048, 1000), (300, 1152, 640), (513, 300, 777), (1171, 4864, 896)]
+
+
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+@pytest.mark.parametrize("n,k,f", SIZES)
+def test_linear(dev, n, k, f, out_dtype):
+    x, sx, w, sw = operands(n, k, f, dev, n + k + f)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = k8.linear_fp8(x, sx, w, sw, out_dtype=out_dtype, status=status)
+    check_linear(out, x, sx, w, sw)
+    assert torch.equal(out, k8.linear_fp8(x, sx, w, sw, out_dtype=out_dtype)) and int(status.item()) == 0
+
+
+@pytest.mark.parametrize("n,k,f", [(5, 300, 200), (70, 512, 390), (260, 1000, 520)])
+def test_linear_into_a_column_range_of_strided_operands(dev, n, k, f):
+    x, sx, w, sw = operands(n, k, f, dev, 5, pad=3)
+    for dtype in (BF, F32):
+        big = torch.full((n + 2, f + 9), 7.0, dtype=dtype, device=dev)
+        k8.linear_fp8(x, sx, w, sw, out_dtype=dtype, out=big[1: n + 1, 4: f + 4])
+        check_linear(big[1: n + 1, 4: f + 4], x, sx, w, sw)
+        big[1: n + 1, 4: f + 4] = 7.0
+        assert (big == 7.0).all()
+
+
+def test_linear_of_single_values(dev):
+    """One value of x and one of w at a time: the product lands where it belongs, with its own block's scales."""
+    n, k, f = 150, 400, 300
+    for t, c, o in [(0, 0, 0), (149, 399, 299), (127, 128, 128), (128, 127, 127), (16, 255, 256), (77, 384, 255)]:
+        x, w = k8.rows_fp8(n, k, dev), k8.rows_fp8(f, k, dev)
+        x.zero_()
+        w.zero_()
+        x[t, c], w[o, c] = 3.5, -20.0
+        sx = torch.arange(1, 4 * n + 1, device=dev, dtype=F32).view(4, n)
+        sw = torch.arange(1, 13, device=dev, dtype=F32).view(3, 4) / 8
+        out = k8.linear_fp8(x, sx, w, sw, out_dtype=F32)
+        want = torch.zeros(n, f)
+        want[t, o] = -70.0 * float(sx[c // 128, t]) * float(sw[o // 128, c // 128])
+        assert torch.equal(out.cpu(), want)
+
+
+def test_linear_rows_do_not_depend_on_their_neighbours(dev):
+    x, sx, w, sw = operands(40, 500, 300, dev, 11)
+    want = k8.linear_fp8(x, sx, w, sw, out_dtype=F32)
+    x[7], x[21, 3] = float("nan"), float("nan")
+    sx[:, 9] = float("inf")
+    got = k8.linear_fp8(x, sx, w, sw, out_dtype=F32)
+    rows = [t for t in range(40) if t not in (7, 21, 9)]
+    assert torch.equal(got[rows], want[rows]) and got[7].isnan().all() and got[21].isnan().all() and not torch.isfinite(got[9]).any()
+
+
+def test_quantized_weights(dev):
+    w = torch.randn(300, 200, generator=gen(3)).to(dev)
+    w[:128, 128:] = 0
+    q, s = k8.quantize_weight(w)
+    assert q.shape == (300, 200) and s.shape == (3, 2) and q.stride(0) % 16 == 0
+    back = q.double().cpu() * s.double().cpu()[torch.arange(300) // 128][:, torch.arange(200) // 128]
+    assert ((back - w.double().cpu()).abs() <= 2.0 ** -4 * (1 + 4 * U) * w.double().cpu().abs() + 2.0 ** -10 * float(s.max())).all()
+
+
+# ---- routes ----------------------------------------------------------------------------------------------------------
+def check_route(r, logits, top, **kw):
+    cpu = {k: (v.cpu() if isinstance(v, torch.Tensor) else v) for k, v in kw.items()}
+    ids, weights, slots, segs = fo.route(logits.cpu(), top, **cpu)
+    assert torch.equal(r.ids.cpu().long(), ids)
+    assert ((r.weights.double().cpu() - weights).abs() <= 2 * U * weights + 1e-44).all()
+    assert torch.equal(r.slots.cpu().long(), slots) and torch.equal(r.segs.cpu().long(), segs)
+
+
+ROUTES = [(1, 16, 2, 1, 1), (1, 1, 1, 1, 1), (3, 5, 5, 1, 1), (64, 256, 8, 8, 4), (33, 60, 4, 1, 1), (257, 64, 6, 8, 3), (40, 160, 6, 8, 3), (9, 384, 8, 1, 1), (7, 1024, 32, 1, 1),
+          (5, 1024, 16, 32, 2), (300, 8, 2, 4, 2), (31, 12, 2, 12, 5), (65, 100, 7, 4, 2), (1000, 37, 3, 1, 1)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("score,biased", [("softmax", False), ("softmax", True), ("sigmoid", False), ("sigmoid", True)])
+@pytest.mark.parametrize("n,experts,top,groups,top_groups", ROUTES)
+def test_route(dev, n, experts, top, groups, top_groups, score, biased, dtype):
+    g = gen(n + experts)
+    logits = (2 * torch.randn(n, experts, generator=g)).to(dtype)
+    bias = 0.1 * torch.randn(experts, generator=g) if biased else None
+    more = dict(score=score, bias=None if bias is None else bias.to(dev), groups=groups, top_groups=top_groups)
+    wide = torch.full((n, experts + 3), 99.0, dtype=dtype, device=dev)
+    wide[:, 1: experts + 1] = logits.to(dev)
+    r = kr.route_by_scores(wide[:, 1: experts + 1], top, **more)
+    check_route(r, logits, top, **more)
+    r = kr.route_by_scores(logits.to(dev), top, renormalize=False, scale=2.5, **more)
+    check_route(r, logits, top, renormalize=False, scale=2.5, **more)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_equal_masked_and_missing_scores(dev, score):
+    inf, nan = float("inf"), float("nan")
+    logits = torch.zeros(12, 8)
+    logits[1] = torch.tensor([1, 2, 2, 1, 2, 1, 2, 0.0])
+    logits[2] = -inf
+    logits[3, :7] = -inf
+    logits[4] = nan
+    logits[5] = torch.tensor([nan, 1, -inf, 3, nan, -inf, 2, nan])
+    logits[6] = torch.tensor([inf, 0, inf, 0, 0, 0, 0, 0])
+    logits[7] = torch.tensor([-inf, -inf, 1, -inf, -inf, -inf, 0.5, -inf])
+    logits[8] = -400.0
+    logits[9] = torch.tensor([80.0, 81, 82, 83, 84, 85, 86, 87]) / 4  # sigmoids that are all 1 or next to it in 32 bits
+    logits[10] = torch.finfo(F32).min
+    logits[11] = torch.tensor([1.0, 1.0000001, 1.0000002, 1, 1, 1, 1, 1])
+    for bias in (None, torch.tensor([0, -inf, 0, nan, 0.5, inf, 0, 0]), torch.full((8,), -3.0)):
+        for groups, top_groups, top in ((1, 1, 4), (4, 2, 4), (2, 1, 3), (8, 3, 3), (4, 4, 8)):
+            for active in (None, torch.tensor([1, 0, 1, 1, 2, 1, 1, 1, 1, -1, 1, 1], dtype=torch.int32)):
+                more = dict(score=score, groups=groups, top_groups=top_groups, bias=None if bias is None else bias.to(dev), active=None if active is None else active.to(dev))
+                check_route(kr.route_by_scores(logits.to(dev), top, **more), logits, top, **more)
+
+
+def test_route_tells_neighbours_of_64_bits_apart(dev):
+    """Scores that are equal in 32 bits and not in 64, and biases that make up for a difference to the last bit but some."""
+    g = gen(5)
+    base = torch.randn(1, 64, generator=g).expand(200, 64)
+    logits = (base + 1e-7 * torch.randn(200, 64, generator=g)).contiguous()
+    bias = -torch.sigmoid(base[0].double()).to(F32)
+    for groups, top_groups in ((1, 1), (8, 2)):
+        more = dict(score="sigmoid", bias=bias.to(dev), groups=groups, top_groups=top_groups)
+        check_route(kr.route_by_scores(logits.to(dev), 8, **more), logits, 8, **more)
+
+
+def test_nothing_is_a_size(dev):
+    q, s = k8.rms_residual_fp8(torch.empty(0, 64, device=dev), torch.ones(64, device=dev), eps=1e-5)
+    assert q.shape == (0, 64) and s.shape == (1, 0)
+    q, s = k8.quantize_fp8(torch.empty(0, 200, dtype=BF, device=dev), "silu_gate")
+    assert q.shape == (0, 100) and s.shape == (1, 0)
+    x, sx, w, sw = operands(1, 64, 10, dev, 1)
+    assert k8.linear_fp8(x[:0], sx[:, :0], w, sw).shape == (0, 10)
+    r = kr.route_by_scores(torch.empty(0, 9, device=dev), 3)
+    assert r.ids.shape == (0, 3) and torch.equal(r.segs.cpu(), torch.zeros(9, 2, dtype=torch.int32))
