@@ -161,7 +161,8 @@ def check_linear(out, x, sx, w, sw):
 
 
 SIZES = [(1, 16, 1), (1, 45, 7), (1, 128, 128), (3, 129, 130), (1, 896, 4864), (16, 256, 300), (17, 384, 129), (31, 1000, 257), (33, 640, 200), (64, 3584, 896),
-         (65, 128, 512), (100, 4864, 130), (128, 512, 128), (129, 1021, 255), (200, 2048, 1000), (300, 1152, 640), (513, 300, 777), (1171, 4864, 896)]
+         (65, 128, 512), (100, 4864, 130), (128, 512, 128), (129, 1021, 255), (200, 2048, 1000), (300, 1152, 640), (513, 300, 777), (1171, 4864, 896), (5, 2100, 300), (64, 2050, 900), (20, 1100, 2000), (130, 2100, 200), (90, 2304, 1100),
+         (2600, 260, 4000), (2563, 130, 4111)]
 
 
 @pytest.mark.parametrize("out_dtype", [BF, F32])
