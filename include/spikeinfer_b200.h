@@ -790,7 +790,7 @@ int spk_linear_fp8(const spk_linear_fp8_args* args, void* stream);
  * active is not 1, get id -1, weight 0 and slot -1.  Comparisons have the outcome of 64-bit arithmetic.
  * slots [n, top] <- row of the (token, choice) pair in the matrix sorted by expert, pairs in their order inside a segment; segs [experts, 2] <- first row
  * and rows of every expert; first rows are multiples of eight (spk_expert_rows, spk_experts).
- * experts <= 1024, top <= 32; workspace of spk_route_scores_workspace_bytes(n, experts) bytes. */
+ * experts <= 1024, top <= 32; workspace of spk_route_scores_workspace_bytes(n, experts) bytes (0: may be NULL). */
 enum {
     SPK_SCORE_SOFTMAX = 0,
     SPK_SCORE_SIGMOID = 1

@@ -12,23 +12,28 @@ from .dense import _call, _f32, _ptr
 
 FP8 = torch.float8_e4m3fn
 BLOCK = 128
+_F32, _BF16 = torch.float32, torch.bfloat16
+_FLOATS = (_F32, _BF16)
 _ACTS = {"none": _lib.ACT_NONE, "gelu_tanh": _lib.ACT_GELU_TANH, "silu_gate": _lib.ACT_SILU_GATE}
 
 
 def rows_fp8(n: int, width: int, device) -> torch.Tensor:
     """An e4m3 ``[n, width]`` matrix, not filled, whose rows start on 16-byte boundaries."""
-    return torch.empty((n, -(-width // 16) * 16), dtype=FP8, device=device)[:, :width]
+    return torch.empty_strided((n, width), (-(-width // 16) * 16, 1), dtype=FP8, device=device)
 
 
 def _is_rows(t: torch.Tensor, what: str) -> None:
-    if t.ndim != 2 or t.dtype != FP8 or t.shape[1] < 1 or t.stride(1) != 1 or t.stride(0) % 16 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
-        raise ValueError(f"{what} must be e4m3 [rows, columns] with unit column stride and rows that start on 16-byte boundaries")
+    if t.ndim == 2 and t.dtype is FP8:
+        (row, column), width = t.stride(), t.shape[1]
+        if column == 1 and row >= width > 0 and not row % 16 and not t.data_ptr() % 16:
+            return
+    raise ValueError(f"{what} must be e4m3 [rows, columns] with unit column stride and rows that start on 16-byte boundaries")
 
 
-def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
+def one_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
+    for t in tensors:
         if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+            raise ValueError(f"all tensors must be on {device}: one is on {t.device}")
 
 
 def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -53,16 +58,16 @@ def rms_residual_fp8(x: torch.Tensor, weight: torch.Tensor, *, eps: float, delta
     ``x`` is fp32 (``delta`` fp32 or bf16) or bf16 (``delta`` bf16), ``pairs`` what :func:`.experts.experts_forward` returned, ``pair_slots`` and
     ``pair_weights`` a route's (:func:`.routing.route_by_scores`); a negative slot adds nothing."""
     _lib.require_cuda(x, "rms_residual_fp8 input")
-    if x.ndim != 2 or not x.is_contiguous() or x.dtype not in (torch.float32, torch.bfloat16):
+    if x.ndim != 2 or not x.is_contiguous() or x.dtype not in _FLOATS:
         raise ValueError("x must be contiguous [n, width], fp32 or bf16")
     n, width = x.shape
     _f32(weight, "weight", width)
     if delta is not None and (delta.shape != x.shape or not delta.is_contiguous()
-                              or delta.dtype not in ((torch.float32, torch.bfloat16) if x.dtype == torch.float32 else (torch.bfloat16,))):
+                              or delta.dtype not in (_FLOATS if x.dtype == _F32 else (_BF16,))):
         raise ValueError("delta must be contiguous and of the shape of x, fp32 or bf16 beside fp32, bf16 beside bf16")
     if x_out is not None and (x_out.shape != x.shape or x_out.dtype != x.dtype or not x_out.is_contiguous()):
         raise ValueError("x_out must be contiguous, of the shape and dtype of x")
-    if out is not None and (out.shape != x.shape or out.dtype not in (torch.float32, torch.bfloat16) or not out.is_contiguous()):
+    if out is not None and (out.shape != x.shape or out.dtype not in _FLOATS or not out.is_contiguous()):
         raise ValueError("out must be contiguous and of the shape of x, fp32 or bf16")
     if pairs is None and (pair_slots is not None or pair_weights is not None):
         raise ValueError("pair_slots and pair_weights name rows of pairs")
@@ -76,9 +81,9 @@ def rms_residual_fp8(x: torch.Tensor, weight: torch.Tensor, *, eps: float, delta
         if pair_weights is None or pair_weights.shape != pair_slots.shape:
             raise ValueError("pair_weights must be [n, top]")
         _f32(pair_weights, "pair_weights")
-    _same_device(x.device, weight=weight, delta=delta, x_out=x_out, out=out, pairs=pairs, pair_slots=pair_slots, pair_weights=pair_weights, status=status)
-    q = rows_fp8(n, width, x.device)
-    scales = torch.empty((-(-width // BLOCK), n), dtype=torch.float32, device=x.device)
+    device = x.device
+    one_device(device, weight, delta, x_out, out, pairs, pair_slots, pair_weights, status)
+    q, scales = rows_fp8(n, width, device), torch.empty((-(-width // BLOCK), n), dtype=_F32, device=device)
     a = _lib.RmsResidualFp8Args(
         x=x.data_ptr(), delta=_ptr(delta), x_out=_ptr(x_out), w=weight.data_ptr(), pairs=_ptr(pairs), pair_slots=_ptr(pair_slots),
         pair_weights=_ptr(pair_weights), out=_ptr(out), q=q.data_ptr(), scales=scales.data_ptr(), pair_rows=0 if pairs is None else pairs.shape[0], n=n,
@@ -95,12 +100,11 @@ def quantize_fp8(z: torch.Tensor, act: str = "none") -> tuple[torch.Tensor, torc
     _lib.require_cuda(z, "quantize_fp8 input")
     if act not in _ACTS:
         raise ValueError(f"unknown activation {act!r} (known: {', '.join(_ACTS)})")
-    if z.ndim != 2 or z.dtype not in (torch.float32, torch.bfloat16) or z.stride(1) != 1 or z.stride(0) < z.shape[1] or z.shape[1] < 1 \
+    if z.ndim != 2 or z.dtype not in _FLOATS or z.stride(1) != 1 or z.stride(0) < z.shape[1] or z.shape[1] < 1 \
             or (act == "silu_gate" and z.shape[1] % 2):
         raise ValueError("z must be [n, width], fp32 or bf16, with unit column stride; an even width for the gate")
     n, width = z.shape[0], z.shape[1] // (2 if act == "silu_gate" else 1)
-    q = rows_fp8(n, width, z.device)
-    scales = torch.empty((-(-width // BLOCK), n), dtype=torch.float32, device=z.device)
+    q, scales = rows_fp8(n, width, z.device), torch.empty((-(-width // BLOCK), n), dtype=_F32, device=z.device)
     a = _lib.QuantizeFp8Args(z=z.data_ptr(), q=q.data_ptr(), scales=scales.data_ptr(), z_stride=z.stride(0), q_stride=q.stride(0), scale_stride=n, n=n,
                              width=width, act=_ACTS[act], dtype=_lib.dtype_code(z.dtype))
     _call("spk_quantize_fp8", a, z.device)
@@ -124,10 +128,10 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("w_scales must be contiguous fp32 [ceil(features / 128), ceil(k / 128)]")
     if out is None:
         out = torch.empty((n, features), dtype=out_dtype, device=x.device)
-    if out.shape != (n, features) or out.dtype != out_dtype or out_dtype not in (torch.float32, torch.bfloat16) or (features > 1 and out.stride(1) != 1) \
+    if out.shape != (n, features) or out.dtype != out_dtype or out_dtype not in _FLOATS or (features > 1 and out.stride(1) != 1) \
             or (n > 1 and out.stride(0) < features):
         raise ValueError("out must be [n, features] in out_dtype, fp32 or bf16, with unit column stride")
-    _same_device(x.device, x_scales=x_scales, w=w, w_scales=w_scales, out=out, status=status)
+    one_device(x.device, x_scales, w, w_scales, out, status)
     a = _lib.LinearFp8Args(x=x.data_ptr(), w=w.data_ptr(), x_scales=x_scales.data_ptr(), w_scales=w_scales.data_ptr(), out=out.data_ptr(),
                            x_stride=x.stride(0), w_stride=w.stride(0), x_scale_stride=max(n, x_scales.stride(0)), w_scale_stride=blocks,
                            out_stride=max(features, out.stride(0)), n=n, k=k, features=features, out_dtype=_lib.dtype_code(out_dtype),

@@ -11,6 +11,7 @@ import torch
 from .. import _lib
 from .dense import _call, _f32, _ptr
 from .experts import LayerRoute
+from .fp8 import one_device
 
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 MAX_EXPERTS, MAX_TOP = 1024, 32
@@ -49,19 +50,18 @@ def route_by_scores(logits: torch.Tensor, top: int, *, score: str = "softmax", b
     _f32(bias, "bias", experts)
     if active is not None and (active.dtype != torch.int32 or active.numel() != n or not active.is_contiguous()):
         raise ValueError("active must be contiguous int32 [n]")
-    for name, t in (("bias", bias), ("active", active)):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"{name} is on {t.device}, not on {logits.device}")
     device = logits.device
-    ids, slots = (torch.empty((n, top), dtype=torch.int32, device=device) for _ in range(2))
-    weights = torch.empty((n, top), dtype=torch.float32, device=device)
+    one_device(device, bias, active)
+    lib = _lib.load()
+    ids, slots, bits = torch.empty((3, n, top), dtype=torch.int32, device=device).unbind(0)  # one allocation: it costs more than a launch
+    weights = bits.view(torch.float32)
     segs = torch.empty((experts, 2), dtype=torch.int32, device=device)
-    need = int(_lib.load().spk_route_scores_workspace_bytes(n, experts))
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    need = int(lib.spk_route_scores_workspace_bytes(n, experts))
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     a = _lib.RouteScoresArgs(
         logits=logits.data_ptr(), bias=_ptr(bias), active=_ptr(active), ids=ids.data_ptr(), weights=weights.data_ptr(), slots=slots.data_ptr(),
-        segs=segs.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=need, logits_stride=max(experts, logits.stride(0)), n=n,
+        segs=segs.data_ptr(), workspace=_ptr(ws), workspace_bytes=need, logits_stride=max(experts, logits.stride(0)), n=n,
         dtype=_lib.dtype_code(logits.dtype), experts=experts, top=top, groups=groups, top_groups=top_groups, score=_SCORES[score],
-        renormalize=int(renormalize), scale=scale)
+        renormalize=renormalize, scale=scale)
     _call("spk_route_scores", a, device)
     return ScoreRoute(slots, segs, ids, weights)

@@ -74,8 +74,8 @@ def test_linear_arguments(lib):
 
 def test_route_arguments(lib):
     fn = lib.spk_route_scores
-    assert lib.spk_route_scores_workspace_bytes(0, 8) == 0 and lib.spk_route_scores_workspace_bytes(33, 8) >= 2 * 8 * 4
-    new = lambda: _lib.RouteScoresArgs(logits=256, ids=256, weights=256, slots=256, segs=256, workspace=256, workspace_bytes=1 << 20, logits_stride=64, n=4, dtype=_lib.F32,
+    assert lib.spk_route_scores_workspace_bytes(0, 8) == 0 and lib.spk_route_scores_workspace_bytes(400, 8) >= 13 * 8 * 4
+    new = lambda: _lib.RouteScoresArgs(logits=256, ids=256, weights=256, slots=256, segs=256, workspace=256, workspace_bytes=1 << 20, logits_stride=64, n=400, dtype=_lib.F32,
                                        experts=64, top=6, groups=8, top_groups=2, score=_lib.SCORE_SIGMOID, renormalize=1, scale=1.0)
     assert fn(None, None) == -4
     for code, changed in ((-2, dict(n=-1)), (-2, dict(experts=0)), (-2, dict(experts=2048)), (-2, dict(top=0)), (-2, dict(top=33)), (-2, dict(groups=7)), (-2, dict(groups=0)),
