@@ -785,12 +785,12 @@ int spk_linear_fp8(const spk_linear_fp8_args* args, void* stream);
 
 /* Experts chosen by scores.  Per token: s = softmax(logits) or 1 / (1 + exp(-logits)), c = s + bias (bias may be NULL).  groups > 1: the experts are cut into
  * `groups` equal runs, a group counts the sum of its best two c, and only the best top_groups groups stay.  ids [n, top] <- the best c in falling order,
- * equal ones by index; weights [n, top] <- s of these, divided by their sum with renormalize (0 where that is 0), times scale.  An expert whose logit or
+ * equal ones by index; weights [n, top] <- s of these, divided by their sum with renormalize (0 where that is 0), times scale, in 32 bits.  An expert whose logit or
  * c is NaN or -infinity is never chosen (+infinity counts as the largest finite 32-bit value); choices that are left over, and all of a token whose
  * active is not 1, get id -1, weight 0 and slot -1.  Comparisons have the outcome of 64-bit arithmetic.
  * slots [n, top] <- row of the (token, choice) pair in the matrix sorted by expert, pairs in their order inside a segment; segs [experts, 2] <- first row
  * and rows of every expert; first rows are multiples of eight (spk_expert_rows, spk_experts).
- * experts <= 1024, top <= 32; workspace of spk_route_scores_workspace_bytes(n, experts) bytes (0: may be NULL). */
+ * experts <= 1024, top <= 32; workspace of spk_route_scores_workspace_bytes(n, experts) bytes (0: may be NULL), 16-byte aligned. */
 enum {
     SPK_SCORE_SOFTMAX = 0,
     SPK_SCORE_SIGMOID = 1

@@ -2,24 +2,33 @@
 //
 // A warp per token, an expert of every 32 per lane.  Choices lie next to borders, where 32 bits would tell equal from unequal by how they were rounded, so they have to
 // come out as in 64-bit arithmetic.  Nearly all of them are settled by 32-bit scores: where every difference that decides (each choice from the next, the worst group kept from
-// the best one dropped) is beyond what the scores can be off by, it has the sign of the exact one.  Tokens with a difference that is not are done again in 64 bits
-// (exact_choice; 64 bits for all of them: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44).  Weights are 64-bit, of the chosen alone where they are divided by their sum.
+// the best one dropped) is beyond what the scores can be off by, it has the sign of the exact one.  Where one is not, the groups, or the experts that can be among the chosen, are
+// compared in 64 bits.  (64 bits for every token: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44; for the whole of a token that is not settled: 49 and 13; so XXX.)
 //
 // A CTA's 32 tokens leave one word per expert, a bit for every token that chose it (a token chooses an expert once).  A pair's row is what the words ahead count, and the
 // bits below its own: no order of arrival enters, so the rows are the same every time.  Up to 256 tokens: a cluster's CTAs read one another's words, one launch.
 // More: score_layout_kernel, from the words in memory.
 #include "spk_experts.cuh"
+#include "spk_tensor.cuh"
 
 namespace {
 
-constexpr int kTokens = 32;        // per CTA of the selection: the bits of a word
+using namespace spk_tc;
+
+constexpr int kTokens = 32;        // per CTA of the selection, at most: the bits of a word
 constexpr int kMostCluster = 8;    // CTAs that hand out the rows among themselves
 constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutWords = 8;    // words per CTA of the layout
 
-// What a 32-bit score can be off by, relative to the score (and to the bias beside it): the exponent's rounding (100 * 2^-24 where the exponential is still normal), the
-// exponential's 2 ulp, 13 sums and a reciprocal are under 2^-17; two of them make a difference.
-constexpr float kOff = 1.52587890625e-5f;  // 2^-16
+// What makes a difference of two 32-bit scores settled: off times the larger (and the bias beside it) and kLeast.  The exponential's argument is off by |x| 2^-23 at most (a product, or a
+// difference and a product), which moves a sigmoid s by s (1 - s) |x| 2^-23 < 2^-25 and a softmax weight by d e^-d 2^-23 < 2^-24 (d: distance from the largest logit): kLeast.  The approximate
+// exponential and reciprocal and the sum under it move s by 2^-21, the sums of a softmax (37 roundings of up to 1024 terms) by 2^-18.6, the bias' addition c by 2^-24, and the
+// bits that a key gives up to the expert's place by 2^-20 (three bits) or 2^-18.  Twice all that for a difference, and up to the next power of two.
+constexpr float kLeast = 2.384185791015625e-7f;  // 2^-22
+__device__ __forceinline__ float off_of(int score, bool key, bool wide) {
+    const float sigmoid = key ? wide ? 1.52587890625e-5f : 3.814697265625e-6f : 9.5367431640625e-7f;  // 2^-16, 2^-18, 2^-20
+    return score == SPK_SCORE_SIGMOID ? sigmoid : wide ? 1.52587890625e-5f : 7.62939453125e-6f;        // 2^-16, 2^-17
+}
 
 __device__ __forceinline__ double warp_max(double v) {
 #pragma unroll
@@ -47,6 +56,13 @@ __device__ __forceinline__ float logit(const T* l, int e) {
 }
 __device__ __forceinline__ int padded(int e) { return e + (e >> 5 << 2); }  // groups of 32 side by side lie in banks of their own
 
+// Lanes for each of up to 32 groups: a power of two.
+__device__ __forceinline__ int lanes_of(int groups) {
+    int L = 32;
+    while (L * groups > 32) L >>= 1;
+    return L;
+}
+
 // The largest logit (0 where there is none) and the sum of the exponentials.
 template <typename T>
 __device__ __noinline__ void exact_softmax(const T* l, int E, double& m, double& sum) {
@@ -59,6 +75,66 @@ __device__ __noinline__ void exact_softmax(const T* l, int E, double& m, double&
     sum = warp_sum(s);
 }
 
+// What the choice goes by, in 64 bits.
+__device__ __forceinline__ double exact_score(const spk_route_scores_args& a, float logit, float bias, double m, double sum) {
+    const double x = logit, v = (a.score == SPK_SCORE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x))) + static_cast<double>(bias);
+    return logit == -INFINITY || v != v ? -INFINITY : v;
+}
+
+// Which groups stay, in 64 bits: a bit for the first lane of each (up to 32 groups).  c: E doubles of shared memory of this warp.
+template <typename T>
+__device__ __noinline__ uint32_t exact_groups(const spk_route_scores_args& a, const T* l, double* c) {
+    const int E = a.experts, lane = threadIdx.x & 31, per = E / a.groups, L = lanes_of(a.groups), g = lane / L;
+    double m = 0.0, sum = 1.0;
+    if (a.score == SPK_SCORE_SOFTMAX) exact_softmax(l, E, m, sum);
+    __syncwarp();
+    for (int e = lane; e < E; e += 32) c[e] = exact_score(a, logit(l, e), a.bias != nullptr ? a.bias[e] : 0.0f, m, sum);
+    __syncwarp();
+    double first = -INFINITY, second = -INFINITY;
+    if (g < a.groups) {
+        for (int k = lane % L; k < per; k += L) {
+            const double v = c[g * per + k];
+            second = fmax(second, fmin(first, v));
+            first = fmax(first, v);
+        }
+    }
+    for (int o = L >> 1; o >= 1; o >>= 1) {
+        const double f = __shfl_xor_sync(~0u, first, o), s = __shfl_xor_sync(~0u, second, o);
+        second = fmax(fmin(first, f), fmax(second, s));
+        first = fmax(first, f);
+    }
+    const double worth = second == -INFINITY ? first : first + second;
+    int better = 0;
+    for (int h = 0; h < a.groups; ++h) {
+        const double w = __shfl_sync(~0u, worth, h * L);
+        better += w > worth || (w == worth && h < g);
+    }
+    __syncwarp();
+    return __ballot_sync(~0u, g < a.groups && better < a.top_groups);
+}
+
+// The order of n <= 32 experts (lane q: list[q]) in 64 bits: lane j gets the j-th of them, -1 where there is none or j >= top.
+template <typename T>
+__device__ __noinline__ int exact_order(const spk_route_scores_args& a, const T* l, const int* list, int n) {
+    const int lane = threadIdx.x & 31, e = lane < n ? list[lane] : 0;
+    double m = 0.0, sum = 1.0;
+    if (a.score == SPK_SCORE_SOFTMAX) exact_softmax(l, a.experts, m, sum);
+    const double c = lane < n ? exact_score(a, logit(l, e), a.bias != nullptr ? a.bias[e] : 0.0f, m, sum) : -INFINITY;
+    int rank = 0;
+    for (int q = 0; q < n; ++q) {
+        const double w = __shfl_sync(~0u, c, q);
+        const int f = __shfl_sync(~0u, e, q);
+        rank += w > c || (w == c && f < e);
+    }
+    if (lane >= n) rank = 32;
+    int mine = -1;
+    for (int j = 0; j < a.top && j < n; ++j) {
+        const int who = __ffs(__ballot_sync(~0u, rank == j)) - 1, got = __shfl_sync(~0u, e, who);
+        if (lane == j) mine = got;
+    }
+    return mine;
+}
+
 // The token's choices in 64 bits: lane j gets choice j, -1 where there is none.  c: 2 E doubles of shared memory of this warp.
 template <typename T>
 __device__ __noinline__ int exact_choice(const spk_route_scores_args& a, const T* l, double* c) {
@@ -67,12 +143,7 @@ __device__ __noinline__ int exact_choice(const spk_route_scores_args& a, const T
     double m = 0.0, sum = 1.0;
     if (a.score == SPK_SCORE_SOFTMAX) exact_softmax(l, E, m, sum);
     __syncwarp();
-    for (int e = lane; e < E; e += 32) {
-        const double x = logit(l, e);
-        double v = a.score == SPK_SCORE_SOFTMAX ? exp(x - m) / sum : 1.0 / (1.0 + exp(-x));
-        if (a.bias != nullptr) v += static_cast<double>(a.bias[e]);
-        c[e] = x == -INFINITY || v != v ? -INFINITY : v;
-    }
+    for (int e = lane; e < E; e += 32) c[e] = exact_score(a, logit(l, e), a.bias != nullptr ? a.bias[e] : 0.0f, m, sum);
     __syncwarp();
     if (a.groups > 1) {
         const int per = E / a.groups;
@@ -114,14 +185,17 @@ __device__ __noinline__ int exact_choice(const spk_route_scores_args& a, const T
     return mine;
 }
 
-// The same by 32-bit scores; false where a difference that decides is too small for them.  x, b: this lane's logits and biases (expert lane + 32 i), c: padded(E) floats.
-template <int P>
-__device__ __forceinline__ bool fast_choice(const spk_route_scores_args& a, const float (&x)[P], const float (&b)[P], float bias_most, float* c, int& mine) {
+// The token's choices.  x, b: this lane's logits and biases (expert lane + 32 i), bit: where a group's bit is, c64: 2 E doubles of shared memory of this warp.  A key's last bits name the
+// expert's place in the lane, the first of equal ones the largest.
+template <typename T, int P>
+__device__ __forceinline__ int choose(const spk_route_scores_args& a, const T* l, const float (&x)[P], const float (&b)[P], const int (&bit)[P], float bias_most, double* c64) {
+    constexpr uint32_t PLACE = P - 1;
+    if (a.groups > 32) return exact_choice(a, l, c64);
     const int E = a.experts, lane = threadIdx.x & 31;
-    uint32_t key[P];
+    float* c = reinterpret_cast<float*>(c64);
+    float v[P];
     {
         float m = 0.0f, scale = 1.0f;
-        float s[P];
         if (a.score == SPK_SCORE_SOFTMAX) {
             m = x[0];
 #pragma unroll
@@ -131,34 +205,31 @@ __device__ __forceinline__ bool fast_choice(const spk_route_scores_args& a, cons
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                s[i] = expf(x[i] - m);
-                sum += s[i];
+                v[i] = ex2((x[i] - m) * 1.4426950408889634f);
+                sum += v[i];
             }
-            scale = 1.0f / spk_warp_sum(sum);
+            scale = rcp(spk_warp_sum(sum));
         }
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const float v = (a.score == SPK_SCORE_SOFTMAX ? s[i] * scale : 1.0f / (1.0f + expf(-x[i]))) + b[i];
-            key[i] = x[i] == -INFINITY || v != v || v == -INFINITY ? 0u : key_of(v);
+            const float y = (a.score == SPK_SCORE_SOFTMAX ? v[i] * scale : sigmoid_fast(x[i])) + b[i];
+            v[i] = x[i] == -INFINITY || y != y ? -INFINITY : y;
         }
     }
-    if (a.groups > 1) {
-        if (a.groups > 32) return false;
-        const int per = E / a.groups;
-        int L = 32;  // lanes of a group: a power of two
-        while (L * a.groups > 32) L >>= 1;
+    if (a.groups > 1 && a.top_groups < a.groups) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < P; ++i)
-            if (lane + 32 * i < E) c[padded(lane + 32 * i)] = key[i] != 0 ? of_key(key[i]) : -INFINITY;
+            if (lane + 32 * i < E) c[padded(lane + 32 * i)] = v[i];
         __syncwarp();
-        const int g = lane / L;
+        const int per = E / a.groups, L = lanes_of(a.groups), g = lane / L;
         float first = -INFINITY, second = -INFINITY;
         if (g < a.groups) {
+#pragma unroll 4
             for (int k = lane % L; k < per; k += L) {
-                const float v = c[padded(g * per + k)];
-                second = fmaxf(second, fminf(first, v));
-                first = fmaxf(first, v);
+                const float y = c[padded(g * per + k)];
+                second = fmaxf(second, fminf(first, y));
+                first = fmaxf(first, y);
             }
         }
         for (int o = L >> 1; o >= 1; o >>= 1) {
@@ -174,78 +245,83 @@ __device__ __forceinline__ bool fast_choice(const spk_route_scores_args& a, cons
         }
         const bool there = g < a.groups, kept = there && better < a.top_groups;
         const float worst = -warp_most(kept ? -worth : -INFINITY), dropped = warp_most(there && !kept ? worth : -INFINITY);
-        if (a.top_groups < a.groups && !(worst - dropped > 2.0f * kOff * (fabsf(worst) + 2.0f * bias_most))) return false;
-        const uint32_t keep = __ballot_sync(~0u, kept);
+        uint32_t keep = __ballot_sync(~0u, kept);
+        if (!(worst - dropped > 2.0f * (off_of(a.score, false, P > 8) * (fabsf(worst) + 2.0f * bias_most) + kLeast))) keep = exact_groups(a, l, c64);
 #pragma unroll
         for (int i = 0; i < P; ++i)
-            if ((keep >> min(31, (lane + 32 * i) / per * L) & 1u) == 0) key[i] = 0;
+            if ((keep >> bit[i] & 1u) == 0) v[i] = -INFINITY;
     }
-    mine = -1;
-    float before = 0.0f;
+    uint32_t key[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) key[i] = v[i] == -INFINITY ? 0u : (key_of(v[i]) & ~PLACE) | (PLACE - i);
+    const float off = off_of(a.score, true, P > 8);
+    int mine = -1, last = 0;
+    float before = 0.0f, apart = 0.0f;
+    bool settled = true;
     for (int j = 0; j <= a.top; ++j) {
         uint32_t most = key[0];
-        int at = 0;
 #pragma unroll
-        for (int i = 1; i < P; ++i)
-            if (key[i] > most) most = key[i], at = i;
+        for (int i = 1; i < P; ++i) most = max(most, key[i]);
         const uint32_t best = __reduce_max_sync(~0u, most);
-        if (best == 0) break;
-        const float v = of_key(best);
-        if (j > 0 && !(before - v > kOff * (fabsf(before) + bias_most))) return false;
-        if (j == a.top) break;
-        const int who = __ffs(__ballot_sync(~0u, most == best)) - 1;
-        const int e = __shfl_sync(~0u, lane + 32 * at, who);
-        if (lane == who) {
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-                if (i == at) key[i] = 0;
+        if (best == 0) {
+            before = -INFINITY;  // everything there is has been chosen
+            break;
         }
+        const int who = __ffs(__ballot_sync(~0u, most == best)) - 1, place = PLACE - static_cast<int>(best & PLACE), e = who + 32 * place;  // equal ones by index
+        const float y = of_key(best & ~PLACE);
+        // experts of the very same logit and bias are equal in 64 bits too
+        if (j > 0 && !(before - y > apart) && (logit(l, last) != logit(l, e) || (a.bias != nullptr && a.bias[last] != a.bias[e]))) settled = false;
+        if (j == a.top) break;
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            if (i == place && lane == who) key[i] = 0;
         if (lane == j) mine = e;
-        before = v;
+        before = y;
+        apart = off * (fabsf(y) + bias_most) + kLeast;
+        last = e;
     }
-    return true;
+    if (settled) return mine;
+    // Those that can be among the chosen, in 64 bits.
+    const float from = before - apart;  // NaN (infinite biases): all of them
+    int* list = reinterpret_cast<int*>(c64);
+    int n = 0;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const bool in = v[i] != -INFINITY && !(v[i] < from);
+        const uint32_t all = __ballot_sync(~0u, in);
+        const int at = n + __popc(all & ((1u << lane) - 1u));
+        if (in && at < 32) list[at] = lane + 32 * i;
+        n += __popc(all);
+    }
+    __syncwarp();
+    return n <= 32 ? exact_order(a, l, list, n) : exact_choice(a, l, c64);
 }
 
-// Adds up what the words of the CTA's tokens and of those ahead count, and lays the segments out.  `word(w, e)`: word w of expert e.  at, before: E integers each; before[e] becomes the
-// row of the first pair of this CTA's tokens (words from w0 on) that chose e.
-template <typename Word>
-__device__ __forceinline__ void lay_out(const spk_route_scores_args& a, int n_words, int w0, bool writes, int32_t* at, int32_t* before, Word word) {
-    const int E = a.experts, threads = blockDim.x;
-    for (int e = threadIdx.x; e < E; e += threads) at[e] = before[e] = 0;
-    __syncthreads();
-    const int wide = E < threads ? E : threads, parts = threads / wide, part = threadIdx.x / wide;
-    if (part < parts) {
-        for (int e = threadIdx.x % wide; e < E; e += wide) {
-            int all = 0, ahead = 0;
-#pragma unroll 8
-            for (int w = part; w < n_words; w += parts) {
-                const int c = __popc(word(w, e));
-                all += c;
-                if (w < w0) ahead += c;
-            }
-            if (all != 0) atomicAdd(at + e, all);
-            if (ahead != 0) atomicAdd(before + e, ahead);
+// Lays the segments out.  at: all pairs of every expert; before: its pairs ahead of this CTA's tokens, which becomes the row of the first pair of theirs.  sums: 32 integers.
+__device__ __forceinline__ void lay_out(const spk_route_scores_args& a, bool writes, const int32_t* at, int32_t* before, int32_t* sums) {
+    const int E = a.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, chunks = (E + 31) / 32;
+    auto scan = [&](int v) {  // of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(~0u, v, o);
+            if (lane >= o) v += up;
         }
+        return v;
+    };
+    auto rows_of = [](int c) { return (c + kExpertAlign - 1) & ~(kExpertAlign - 1); };
+    for (int k = warp; k < chunks; k += warps) {
+        const int upto = scan(32 * k + lane < E ? rows_of(at[32 * k + lane]) : 0);
+        if (lane == 31) sums[k] = upto;
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        int rows = 0;
-        for (int e0 = 0; e0 < E; e0 += 32) {
-            const int e = e0 + threadIdx.x;
-            const int c = e < E ? at[e] : 0;
-            const int pad = (c + kExpertAlign - 1) & ~(kExpertAlign - 1);
-            int upto = pad;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(~0u, upto, o);
-                if (static_cast<int>(threadIdx.x) >= o) upto += up;
-            }
-            if (e < E) {
-                const int first = rows + upto - pad;
-                before[e] += first;
-                if (writes) reinterpret_cast<int2*>(a.segs)[e] = make_int2(first, c);
-            }
-            rows += __shfl_sync(~0u, upto, 31);
+    const int mine = lane < chunks ? sums[lane] : 0, ahead = scan(mine) - mine;  // of chunk `lane`
+    for (int k = warp; k < chunks; k += warps) {
+        const int e = 32 * k + lane, c = e < E ? at[e] : 0, rows = rows_of(c);
+        const int first = __shfl_sync(~0u, ahead, k) + scan(rows) - rows;
+        if (e < E) {
+            before[e] += first;
+            if (writes) reinterpret_cast<int2*>(a.segs)[e] = make_int2(first, c);
         }
     }
     __syncthreads();
@@ -260,13 +336,13 @@ __device__ __forceinline__ uint32_t cluster_load(const uint32_t* p, uint32_t ran
 
 // WHOLE: the grid is one cluster and hands out the rows as well.
 template <typename T, int P, bool WHOLE>
-__global__ void __launch_bounds__(1024)
-score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* words, const int n_words) {
+__global__ void __launch_bounds__(WHOLE ? 1024 : 512)
+score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* words, const int n_words, const int tokens) {
     extern __shared__ double sm[];
     const int E = a.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     double* c64 = sm + static_cast<int64_t>(warp) * 2 * E;  // also the 32-bit scores
     uint32_t* word = reinterpret_cast<uint32_t*>(sm + static_cast<int64_t>(warps) * 2 * E);
-    int32_t* chosen = reinterpret_cast<int32_t*>(word + E);  // WHOLE: [32][top], then 2 E integers
+    int32_t* chosen = reinterpret_cast<int32_t*>(word + E);  // WHOLE: [32][top], then 2 E + 32 integers
     for (int e = threadIdx.x; e < E; e += blockDim.x) word[e] = 0;
     float b[P], bias_most = 0.0f;
 #pragma unroll
@@ -275,56 +351,81 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
         if (fabsf(b[i]) < INFINITY) bias_most = fmaxf(bias_most, fabsf(b[i]));
     }
     bias_most = warp_most(bias_most);
+    int bit[P];
+    const int per = E / a.groups, L = a.groups <= 32 ? lanes_of(a.groups) : 1;
+#pragma unroll
+    for (int i = 0; i < P; ++i) bit[i] = min(31, (lane + 32 * i) / per * L);
     __syncthreads();
-    for (int i = warp; i < kTokens; i += warps) {
-        const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + i;
+    for (int i = warp; i < tokens; i += warps) {
+        const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + i;
         if (t >= a.n) break;
         int mine = -1;  // choice number `lane` of the token
         const T* l = static_cast<const T*>(a.logits) + t * a.logits_stride;
-        double s = 0.0;
+        float s = 0.0f;
         if (a.active == nullptr || a.active[t] == 1) {
             float x[P];
 #pragma unroll
             for (int k = 0; k < P; ++k) x[k] = lane + 32 * k < E ? logit(l, lane + 32 * k) : -INFINITY;
-            if (!fast_choice<P>(a, x, b, bias_most, reinterpret_cast<float*>(c64), mine)) mine = exact_choice(a, l, c64);
+            mine = choose<T, P>(a, l, x, b, bit, bias_most, c64);
             if (mine >= 0) atomicOr(word + mine, 1u << i);
-            const double y = mine >= 0 ? static_cast<double>(logit(l, mine)) : 0.0;
+            // 32-bit weights, every exponent at most zero.  sigmoid(y) = exp(min(y, 0)) / (1 + exp(-|y|)).  Where they are divided by their sum, a factor of all of them falls out (the sum of a
+            // softmax too): the exponents count from the largest of the chosen, unless 64 bits would have had nothing left of it.
+            const float y = mine >= 0 ? logit(l, mine) : -INFINITY;
+            float m = 0.0f;
             if (a.score == SPK_SCORE_SIGMOID) {
-                s = 1.0 / (1.0 + exp(-y));
-            } else if (a.renormalize) {  // the sum over all experts falls out of the quotient
-                float top = x[0];
+                if (a.renormalize) m = warp_most(fminf(y, 0.0f));
+                s = m < -745.0f ? 0.0f : expf(fminf(y, 0.0f) - m) / (1.0f + expf(-fabsf(y)));
+            } else {
+                float top = x[0], sum = 0.0f;
 #pragma unroll
                 for (int k = 1; k < P; ++k) top = fmaxf(top, x[k]);
                 top = warp_most(top);
-                s = exp(y - (top == -INFINITY ? 0.0 : static_cast<double>(top)));
-            } else {
-                double m, sum;
-                exact_softmax(l, E, m, sum);
-                s = exp(y - m) / sum;
+                m = a.renormalize ? warp_most(y) : top;
+                s = m - top < -745.0f ? 0.0f : expf(y - m);
+                if (!a.renormalize) {
+#pragma unroll
+                    for (int k = 0; k < P; ++k) sum += expf(x[k] - m);
+                    s /= spk_warp_sum(sum);
+                }
             }
-            if (mine < 0) s = 0.0;
+            if (mine < 0) s = 0.0f;
             if (a.renormalize) {
-                const double sum = warp_sum(s);
-                s = sum > 0.0 ? s / sum : 0.0;
+                const float sum = spk_warp_sum(s);
+                s = sum > 0.0f ? s / sum : 0.0f;
             }
         }
         if (lane < a.top) {
             a.ids[t * a.top + lane] = mine;
-            a.weights[t * a.top + lane] = static_cast<float>(s * static_cast<double>(a.scale));
+            a.weights[t * a.top + lane] = s * a.scale;
             if (WHOLE) chosen[i * a.top + lane] = mine;
         }
     }
     __syncthreads();
     if (!WHOLE) {
-        for (int e = threadIdx.x; e < E; e += blockDim.x) words[static_cast<int64_t>(blockIdx.x) * E + e] = word[e];
+        // [expert][word], whole 16 bytes of them
+        const int row = (n_words + 3) & ~3, behind = blockIdx.x + 1 == n_words ? row - n_words : 0;
+        for (int e = threadIdx.x; e < E; e += blockDim.x)
+            for (int k = 0; k <= behind; ++k) words[static_cast<int64_t>(e) * row + blockIdx.x + k] = k == 0 ? word[e] : 0u;
         return;
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     int32_t *at = chosen + kTokens * a.top, *before = at + E;
-    lay_out(a, n_words, blockIdx.x, blockIdx.x == 0, at, before, [&](int w, int e) { return cluster_load(word + e, w); });
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        int all = 0, ahead = 0;
+#pragma unroll
+        for (int w = 0; w < kMostCluster; ++w) {
+            const int c = w < n_words ? __popc(cluster_load(word + e, w)) : 0;
+            all += c;
+            if (w < static_cast<int>(blockIdx.x)) ahead += c;
+        }
+        at[e] = all;
+        before[e] = ahead;
+    }
+    __syncthreads();
+    lay_out(a, blockIdx.x == 0, at, before, before + E);
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' words have been read
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens;
-    const int pairs = static_cast<int>(min(a.n - first, static_cast<int64_t>(kTokens))) * a.top;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens;
+    const int pairs = static_cast<int>(min(a.n - first, static_cast<int64_t>(tokens))) * a.top;
     for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
         const int e = chosen[i];
         a.slots[first * a.top + i] = e >= 0 ? before[e] + __popc(word[e] & ((1u << (i / a.top)) - 1u)) : -1;
@@ -334,24 +435,44 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
 
 __global__ void __launch_bounds__(kLayoutThreads)
 score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ words, const int n_words) {
-    extern __shared__ int32_t sm32[];
-    const int E = a.experts, w0 = blockIdx.x * kLayoutWords;
+    extern __shared__ int32_t sm32[];  // [experts] twice, 32
+    const int E = a.experts, w0 = blockIdx.x * kLayoutWords, row = (n_words + 3) & ~3, quads = row / 4;
     int32_t *at = sm32, *before = at + E;
+    for (int e = threadIdx.x; e < 2 * E; e += kLayoutThreads) sm32[e] = 0;
+    __syncthreads();
     spk_grid_wait();
-    lay_out(a, n_words, w0, blockIdx.x == 0, at, before, [&](int w, int e) { return __ldcg(words + static_cast<int64_t>(w) * E + e); });
-    const int64_t lo = static_cast<int64_t>(w0) * kTokens * a.top, hi = min(lo + static_cast<int64_t>(kLayoutWords) * kTokens * a.top, a.n * a.top);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kLayoutThreads) {
-        const int e = __ldcg(a.ids + i);
+    auto load = [&](int e, int q) { return __ldcg(reinterpret_cast<const uint4*>(words + static_cast<int64_t>(e) * row) + q); };
+    auto count = [](const uint4& u, int n) {  // of the first n words
+        return (n > 0 ? __popc(u.x) : 0) + (n > 1 ? __popc(u.y) : 0) + (n > 2 ? __popc(u.z) : 0) + (n > 3 ? __popc(u.w) : 0);
+    };
+    // lanes side by side take a row's words, 16 bytes each: 16 loads of 1024 threads bring 8192 tokens' words of 256 experts
+    const int side = quads < 32 ? quads < 4 ? 1 : quads < 16 ? 4 : 16 : 32;
+    for (int e = threadIdx.x / side; e < E; e += kLayoutThreads / side) {
+        int all = 0, ahead = 0;
+#pragma unroll 4
+        for (int q = threadIdx.x % side; q < quads; q += side) {
+            const uint4 u = load(e, q);
+            const int c = count(u, 4);
+            all += c;
+            if (4 * q < w0) ahead += c;  // w0 is a multiple of four
+        }
+        if (all != 0) atomicAdd(at + e, all);
+        if (ahead != 0) atomicAdd(before + e, ahead);
+    }
+    __syncthreads();
+    lay_out(a, blockIdx.x == 0, at, before, before + E);
+    const int64_t lo = static_cast<int64_t>(w0) * kTokens * a.top;
+    const int pairs = static_cast<int>(min(static_cast<int64_t>(kLayoutWords) * kTokens, a.n - static_cast<int64_t>(w0) * kTokens)) * a.top;
+    for (int i = threadIdx.x; i < pairs; i += kLayoutThreads) {
+        const int e = __ldcg(a.ids + lo + i);
         int slot = -1;
         if (e >= 0) {
-            const int64_t t = i / a.top;
-            const int w = static_cast<int>(t / kTokens);
-            slot = before[e] + __popc(__ldcg(words + static_cast<int64_t>(w) * E + e) & ((1u << (t % kTokens)) - 1u));
-#pragma unroll
-            for (int v = 0; v < kLayoutWords - 1; ++v)
-                if (w0 + v < w) slot += __popc(__ldcg(words + static_cast<int64_t>(w0 + v) * E + e));
+            const int t = i / a.top, w = t / kTokens;  // word of the CTA's
+            const uint4 u = load(e, w0 / 4), v = w0 / 4 + 1 < quads ? load(e, w0 / 4 + 1) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t own = w < 4 ? (w < 2 ? (w == 0 ? u.x : u.y) : (w == 2 ? u.z : u.w)) : (w < 6 ? (w == 4 ? v.x : v.y) : (w == 6 ? v.z : v.w));
+            slot = before[e] + __popc(own & ((1u << (t % kTokens)) - 1u)) + count(u, w) + count(v, w - 4);
         }
-        a.slots[i] = slot;
+        a.slots[lo + i] = slot;
     }
 }
 
@@ -359,9 +480,12 @@ int64_t words_of(int64_t n) { return (n + kTokens - 1) / kTokens; }
 
 template <typename T, int P, bool WHOLE>
 int launch_select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStream_t s) {
-    // 64-bit scores of a warp are kept in shared memory: as many warps as fit, 32 where few CTAs make the grid
-    const int per = 16 * a.experts, extra = 4 * a.experts + (WHOLE ? 4 * (kTokens * a.top + 2 * a.experts) : 0);
-    int warps = WHOLE || n_words <= 148 ? 32 : 16;
+    // a cluster of eight CTAs shares few tokens evenly (64 rows of 256 experts: XXX us, 19.4 as two CTAs of 32)
+    const int tokens = WHOLE ? static_cast<int>((a.n + kMostCluster - 1) / kMostCluster) : kTokens;
+    if (WHOLE) n_words = static_cast<int>((a.n + tokens - 1) / tokens);
+    // 64-bit scores of a warp are kept in shared memory: as many warps as fit
+    const int per = 16 * a.experts, extra = 4 * a.experts + (WHOLE ? 4 * (kTokens * a.top + 2 * a.experts + 32) : 0);
+    int warps = !WHOLE ? 16 : tokens < 8 ? 8 : tokens;  // eight at least hand out the rows
     while (warps * per + extra > 200 * 1024) warps /= 2;
     const int bytes = warps * per + extra;
     auto kernel = score_select_kernel<T, P, WHOLE>;
@@ -377,7 +501,7 @@ int launch_select(const spk_route_scores_args& a, uint32_t* words, int n_words, 
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = WHOLE ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kernel, a, words, n_words);
+    e = cudaLaunchKernelEx(&cfg, kernel, a, words, n_words, tokens);
     if (e != cudaSuccess) return spk_set_cuda_error(e);
     spk_count_launch();
     return SPK_OK;
@@ -397,7 +521,7 @@ int select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStr
 
 extern "C" int64_t spk_route_scores_workspace_bytes(int64_t n, int experts) {
     if (n <= kMostCluster * kTokens || experts < 1) return 0;
-    return words_of(n) * experts * static_cast<int64_t>(sizeof(uint32_t));
+    return (words_of(n) + 3) / 4 * 16 * experts;
 }
 
 extern "C" int spk_route_scores(const spk_route_scores_args* args, void* stream) {
@@ -419,9 +543,10 @@ extern "C" int spk_route_scores(const spk_route_scores_args* args, void* stream)
         if (a.logits_stride < a.experts) return SPK_ERR_BAD_STRIDE;
         if (n_words <= kMostCluster) return a.dtype == SPK_F32 ? select<float, true>(a, words, n_words, s) : select<__nv_bfloat16, true>(a, words, n_words, s);
         if (a.workspace == nullptr || a.workspace_bytes < spk_route_scores_workspace_bytes(a.n, a.experts)) return SPK_ERR_WORKSPACE_TOO_SMALL;
+        if (reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) return SPK_ERR_BAD_STRIDE;
         const int rc = a.dtype == SPK_F32 ? select<float, false>(a, words, n_words, s) : select<__nv_bfloat16, false>(a, words, n_words, s);
         if (rc != SPK_OK) return rc;
     }
     const int grid = n_words == 0 ? 1 : (n_words + kLayoutWords - 1) / kLayoutWords;
-    return spk_launch(score_layout_kernel, dim3(grid), kLayoutThreads, 2 * sizeof(int32_t) * a.experts, s, n_words > 0, a, words, n_words);
+    return spk_launch(score_layout_kernel, dim3(grid), kLayoutThreads, sizeof(int32_t) * (2 * a.experts + 32), s, n_words > 0, a, words, n_words);
 }

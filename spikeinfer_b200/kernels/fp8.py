@@ -22,6 +22,10 @@ def rows_fp8(n: int, width: int, device) -> torch.Tensor:
     return torch.empty_strided((n, width), (-(-width // 16) * 16, 1), dtype=FP8, device=device)
 
 
+def _scales(n: int, width: int, device) -> torch.Tensor:
+    return torch.empty_strided((-(-width // BLOCK), n), (n, 1), dtype=_F32, device=device)
+
+
 def _is_rows(t: torch.Tensor, what: str) -> None:
     if t.ndim == 2 and t.dtype is FP8:
         (row, column), width = t.stride(), t.shape[1]
@@ -83,7 +87,7 @@ def rms_residual_fp8(x: torch.Tensor, weight: torch.Tensor, *, eps: float, delta
         _f32(pair_weights, "pair_weights")
     device = x.device
     one_device(device, weight, delta, x_out, out, pairs, pair_slots, pair_weights, status)
-    q, scales = rows_fp8(n, width, device), torch.empty((-(-width // BLOCK), n), dtype=_F32, device=device)
+    q, scales = rows_fp8(n, width, device), _scales(n, width, device)
     a = _lib.RmsResidualFp8Args(
         x=x.data_ptr(), delta=_ptr(delta), x_out=_ptr(x_out), w=weight.data_ptr(), pairs=_ptr(pairs), pair_slots=_ptr(pair_slots),
         pair_weights=_ptr(pair_weights), out=_ptr(out), q=q.data_ptr(), scales=scales.data_ptr(), pair_rows=0 if pairs is None else pairs.shape[0], n=n,
@@ -104,7 +108,7 @@ def quantize_fp8(z: torch.Tensor, act: str = "none") -> tuple[torch.Tensor, torc
             or (act == "silu_gate" and z.shape[1] % 2):
         raise ValueError("z must be [n, width], fp32 or bf16, with unit column stride; an even width for the gate")
     n, width = z.shape[0], z.shape[1] // (2 if act == "silu_gate" else 1)
-    q, scales = rows_fp8(n, width, z.device), torch.empty((-(-width // BLOCK), n), dtype=_F32, device=z.device)
+    q, scales = rows_fp8(n, width, z.device), _scales(n, width, z.device)
     a = _lib.QuantizeFp8Args(z=z.data_ptr(), q=q.data_ptr(), scales=scales.data_ptr(), z_stride=z.stride(0), q_stride=q.stride(0), scale_stride=n, n=n,
                              width=width, act=_ACTS[act], dtype=_lib.dtype_code(z.dtype))
     _call("spk_quantize_fp8", a, z.device)
