@@ -336,7 +336,7 @@ __device__ __forceinline__ uint32_t cluster_load(const uint32_t* p, uint32_t ran
 
 // WHOLE: the grid is one cluster and hands out the rows as well.
 template <typename T, int P, bool WHOLE>
-__global__ void __launch_bounds__(WHOLE ? 1024 : 512)
+__global__ void __launch_bounds__(WHOLE ? 1024 : 512, WHOLE ? 1 : 2)
 score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* words, const int n_words, const int tokens) {
     extern __shared__ double sm[];
     const int E = a.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;

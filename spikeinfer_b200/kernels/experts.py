@@ -47,15 +47,22 @@ def _blocks(w: torch.Tensor, per: int) -> torch.Tensor:
 
 
 class ExpertWeights:
-    """Gate, up and down matrices of a layer's experts in the layout of their kernels, and the table that names a token's experts."""
+    """Gate, up and down matrices of a layer's experts in the layout of their kernels, and the table that names a token's experts; without one
+    (``top`` experts a token) the layer is routed by scores (:func:`.routing.route_by_scores`)."""
 
-    def __init__(self, gates, ups, downs, table: torch.Tensor) -> None:
+    def __init__(self, gates, ups, downs, table: torch.Tensor | None = None, top: int | None = None) -> None:
         self.experts, self.ff, self.width = len(gates), gates[0].shape[0], gates[0].shape[1]
-        self.top = table.shape[1]
         dtype, device = gates[0].dtype, gates[0].device
-        if int(table.min()) < 0 or int(table.max()) >= self.experts:
-            raise ValueError("the expert table names experts that do not exist")
-        self.table = table.to(device=device, dtype=torch.int32).contiguous()
+        if (table is None) == (top is None):
+            raise ValueError("either a table that names a token's experts, or how many scores choose")
+        self.top, self.table = top, None
+        if table is None:
+            if not 1 <= top <= self.experts:
+                raise ValueError(f"{top} of {self.experts} experts")
+        else:
+            if int(table.min()) < 0 or int(table.max()) >= self.experts:
+                raise ValueError("the expert table names experts that do not exist")
+            self.top, self.table = table.shape[1], table.to(device=device, dtype=torch.int32).contiguous()
         self.dtype, self.tiled = dtype, dtype == torch.bfloat16
         if self.tiled:
             # [experts][blocks][ktiles][gate | up][128][64] and [experts][blocks][ktiles][256][64]
@@ -93,7 +100,7 @@ class ExpertRouter:
         self.layers, self.vocab = layers, vocab
         rows, self.tops, self.entries = [], 0, 0
         for w in layers:
-            if w.table.shape[0] != vocab:
+            if w.table is None or w.table.shape[0] != vocab:
                 raise ValueError("the expert table needs one row per token id")
             rows.append([w.table.data_ptr(), w.top, w.experts, self.tops, 2 * self.entries, 0, 0, 0])
             self.tops += w.top
@@ -119,7 +126,9 @@ def experts_forward(x: torch.Tensor, w: ExpertWeights, route: LayerRoute, status
     """Every expert's feed-forward on its rows of the sorted matrix ``x``: fp32 ``[rows, width]``, unweighted.  ``beside``: another stream's launches run at
     the same time and should find SMs free (the products alone take longer then)."""
     _lib.require_cuda(x, "experts_forward input")
-    n = route.slots.shape[0]
+    n, top = route.slots.shape
+    if top != w.top or route.segs.shape[0] != w.experts:
+        raise ValueError(f"a route of {top} of {route.segs.shape[0]} experts for a layer of {w.top} of {w.experts}")
     rows = w.rows(n)
     hidden = w.sorted_matrix(n, w.ff)
     out = torch.empty((rows, w.width), dtype=torch.float32, device=x.device)

@@ -8,6 +8,8 @@ import torch
 
 from oracle import fp8_oracle as fo
 from spikeinfer_b200 import _lib
+from spikeinfer_b200.kernels import dense as kn
+from spikeinfer_b200.kernels import experts as ke
 from spikeinfer_b200.kernels import fp8 as k8
 from spikeinfer_b200.kernels import routing as kr
 
@@ -295,3 +297,126 @@ def test_nothing_is_a_size(dev):
     assert k8.linear_fp8(x[:0], sx[:, :0], w, sw).shape == (0, 10)
     r = kr.route_by_scores(torch.empty(0, 9, device=dev), 3)
     assert r.ids.shape == (0, 3) and torch.equal(r.segs.cpu(), torch.zeros(9, 2, dtype=torch.int32))
+
+
+# ---- together --------------------------------------------------------------------------------------------------------
+def rel(got, want) -> float:
+    return float((got.double().cpu() - want).pow(2).mean().sqrt() / want.pow(2).mean().sqrt().clamp(min=1e-30))
+
+
+class Block:
+    """A pre-norm block with an 8-bit dense feed-forward and, beside it, experts chosen by scores."""
+
+    def __init__(self, dev, width=256, ff=384, experts=16, top=3, eff=72, seed=1):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        rnd = lambda *s: torch.randn(*s, generator=g, device=dev)
+        self.width, self.top = width, top
+        self.w1, self.w2 = 1 + 0.2 * rnd(width), 1 + 0.2 * rnd(width)
+        self.up, self.down = k8.quantize_weight(rnd(ff, width) / width ** 0.5), k8.quantize_weight(rnd(width, ff) / ff ** 0.5)
+        self.router, self.bias = rnd(experts, width) / width ** 0.5, 0.05 * rnd(experts)
+        self.parts = [[(rnd(*s) / s[1] ** 0.5).to(BF) for _ in range(experts)] for s in ((eff, width), (eff, width), (width, eff))]
+        self.experts = ke.ExpertWeights(*self.parts, top=top)
+
+    def run(self, x, delta, status):
+        n, s = x.shape[0], {}
+        s["x1"], s["h"] = torch.empty_like(x), torch.empty(n, self.width, dtype=BF, device=x.device)
+        s["q1"], s["s1"] = k8.rms_residual_fp8(x, self.w1, eps=1e-5, delta=delta, x_out=s["x1"], out=s["h"], status=status)
+        s["z"] = k8.linear_fp8(s["q1"], s["s1"], *self.up, status=status)
+        s["q2"], s["s2"] = k8.quantize_fp8(s["z"], "gelu_tanh")
+        s["ff"] = k8.linear_fp8(s["q2"], s["s2"], *self.down, out_dtype=F32, status=status)
+        s["logits"] = s["h"].float() @ self.router.t()
+        r = s["route"] = kr.route_by_scores(s["logits"], self.top, score="sigmoid", bias=self.bias, groups=4, top_groups=2)
+        rows = self.experts.sorted_matrix(n, self.width)
+        kn.rms_residual(x=s["x1"], w2=self.w1, eps=1e-5, out2=rows, out2_slots=r.slots, out2_tiled=self.experts.tiled, status=status)
+        s["pairs"] = ke.experts_forward(rows, self.experts, r, status)
+        s["x2"] = torch.empty_like(x)
+        s["q3"], s["s3"] = k8.rms_residual_fp8(s["x1"], self.w2, eps=1e-5, delta=s["ff"], x_out=s["x2"], pairs=s["pairs"], pair_slots=r.slots, pair_weights=r.weights,
+                                               status=status)
+        return s
+
+
+@pytest.mark.parametrize("n", [1, 6, 70, 300])
+def test_a_block_of_them(dev, n):
+    block = Block(dev)
+    g = torch.Generator(device=dev).manual_seed(n)
+    x, delta = torch.randn(n, block.width, generator=g, device=dev), torch.randn(n, block.width, generator=g, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    s = block.run(x, delta, status)
+    assert int(status.item()) == 0
+    c = {k: v.cpu() for k, v in s.items() if isinstance(v, torch.Tensor)}
+    holds8(s["q1"], s["s1"], fo.rms_norm(c["x1"], block.w1.cpu(), 1e-5), NORM)
+    check_linear(s["z"], s["q1"], s["s1"], *block.up)
+    check_linear(s["ff"], s["q2"], s["s2"], *block.down)
+    check_route(s["route"], s["logits"], block.top, score="sigmoid", bias=block.bias, groups=4, top_groups=2)
+    # the experts' products by token, on the norm as it was rounded for them
+    h, r = c["h"].double(), s["route"]
+    gates, ups, downs = ([w.double().cpu() for w in part] for part in block.parts)
+    want = fo.boundary(c["x1"], c["ff"])
+    for t in range(n):
+        for j in range(block.top):
+            e = int(r.ids[t, j])
+            y = h[t] @ gates[e].t()
+            want[t] += float(r.weights[t, j]) * ((y / (1 + torch.exp(-y)) * (h[t] @ ups[e].t())).to(BF).double() @ downs[e].t())
+    assert rel(s["x2"], want) < 4e-3  # the experts' inner products are rounded to bf16, 2^-8 each at most, and are a part of the sum
+    holds8(s["q3"], s["s3"], fo.rms_norm(c["x2"], block.w2.cpu(), 1e-5), NORM)
+
+
+def test_a_captured_block_and_one_beside_it(dev):
+    """A captured block replayed on new inputs, while another stream runs the same operators: both as if alone."""
+    block, other = Block(dev, seed=1), Block(dev, seed=2)
+    new = lambda n, seed: torch.randn(n, block.width, generator=torch.Generator(device=dev).manual_seed(seed), device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    n = 300
+    x, delta = new(n, 1), new(n, 2)
+    block.run(x, delta, status)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = block.run(x, delta, status)
+    keep = ("x2", "q3", "s3", "ff", "pairs")
+    bits = lambda t: t.contiguous().view(torch.uint8)
+    alone = {}
+    for seed in (5, 6):
+        alone[seed] = {k: v.clone() for k, v in block.run(new(n, seed), new(n, seed + 50), status).items() if k in ("x2", "q3", "s3", "ff")}
+    y = new(40, 9), new(40, 10)
+    quiet = other.run(*y, status)["x2"].clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for seed in (5, 6, 5):
+        x.copy_(new(n, seed))
+        delta.copy_(new(n, seed + 50))
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = [other.run(*y, status)["x2"] for _ in range(5)]
+        torch.cuda.synchronize()
+        for k, want in alone[seed].items():
+            assert torch.equal(bits(held[k]), bits(want)), k
+        assert all(torch.equal(b, quiet) for b in beside)
+    assert int(status.item()) == 0 and keep
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------
+def test_refusals(dev):
+    x, w = torch.randn(4, 48, device=dev), torch.ones(48, device=dev)
+    slots, weights, pairs = torch.zeros(4, 2, dtype=torch.int32, device=dev), torch.ones(4, 2, device=dev), torch.randn(8, 48, device=dev)
+    b = lambda **k: (lambda: k8.rms_residual_fp8(**(dict(x=x, weight=w, eps=1e-5) | k)))
+    q, s = k8.quantize_fp8(x)
+    qw, sw = k8.quantize_weight(torch.randn(10, 48, device=dev))
+    f = lambda **k: (lambda: k8.linear_fp8(**(dict(x=q, x_scales=s, w=qw, w_scales=sw) | k)))
+    r = lambda logits=torch.randn(4, 12, device=dev), top=3, **k: (lambda: kr.route_by_scores(logits, top, **k))
+    experts = lambda **k: (lambda: ke.ExpertWeights([pairs] * 4, [pairs] * 4, [pairs.t().contiguous()] * 4, **k))
+    for call in (b(x=x.half()), b(x=x[:, ::2]), b(x=x[0]), b(weight=w[:47]), b(weight=w.to(BF)), b(delta=x[:3]), b(delta=x.half()), b(x=x.to(BF), delta=x), b(x_out=x.to(BF)),
+                 b(x_out=torch.empty(4, 96, device=dev)[:, ::2]), b(out=x.half()), b(pairs=pairs), b(pairs=pairs, pair_slots=slots), b(pair_weights=weights),
+                 b(pairs=pairs, pair_slots=slots.long(), pair_weights=weights), b(pairs=pairs, pair_slots=slots[:3], pair_weights=weights[:3]),
+                 b(pairs=pairs, pair_slots=slots, pair_weights=weights[:, :1]), b(pairs=pairs[:, :40], pair_slots=slots, pair_weights=weights), b(delta=x.cpu()),
+                 lambda: k8.quantize_fp8(x, "relu"), lambda: k8.quantize_fp8(x.half()), lambda: k8.quantize_fp8(x.t()), lambda: k8.quantize_fp8(x[:, :47], "silu_gate"),
+                 f(x=x), f(x=q[:, :40]), f(x=q[:, 1:]), f(w=qw.t()), f(x_scales=s.t()), f(x_scales=s.double()), f(x_scales=s[:, :3]), f(w_scales=sw.t().contiguous().expand(2, 1)),
+                 f(out_dtype=torch.float16), f(out=torch.empty(4, 10, device=dev)), f(out=torch.empty(4, 20, dtype=BF, device=dev)[:, ::2]), f(w=qw.cpu()), f(x_scales=s.cpu()),
+                 r(top=0), r(top=13), r(top=33), r(logits=torch.randn(4, 2000, device=dev)), r(logits=torch.randn(4, 12, device=dev).half()), r(logits=torch.randn(12, 4, device=dev).t()),
+                 r(score="tanh"), r(groups=5), r(groups=4, top_groups=5), r(groups=4, top_groups=0), r(groups=6, top_groups=1), r(bias=torch.zeros(11, device=dev)),
+                 r(bias=torch.zeros(12, device=dev).to(BF)), r(bias=torch.zeros(12)), r(active=torch.ones(4, device=dev)), r(active=torch.ones(3, dtype=torch.int32, device=dev)),
+                 experts(), experts(top=0), experts(top=5), experts(top=2, table=torch.zeros(9, 2, dtype=torch.int64, device=dev)),
+                 lambda: ke.experts_forward(pairs, experts(top=2)(), kr.route_by_scores(torch.randn(4, 4, device=dev), 3)),
+                 lambda: ke.ExpertRouter([experts(top=2)()], 9)):
+        with pytest.raises((ValueError, TypeError)):
+            call()
