@@ -3,7 +3,9 @@
 // A warp per token, an expert of every 32 per lane.  Choices lie next to borders, where 32 bits would tell equal from unequal by how they were rounded, so they have to
 // come out as in 64-bit arithmetic.  Nearly all of them are settled by 32-bit scores: where every difference that decides (each choice from the next, the worst group kept from
 // the best one dropped) is beyond what the scores can be off by, it has the sign of the exact one.  Where one is not, the groups, or the experts that can be among the chosen, are
-// compared in 64 bits.  (64 bits for every token: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44; for the whole of a token that is not settled: 49 and 13; so XXX.)
+// compared in 64 bits.  (64 bits for every token: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44; for the whole of a token that is not settled: 49 and 13; so 39 and 9.5.)
+//
+// What bounds it: some 1300 instructions a token (scores 200, groups 250, choices 500, weights 100) and their latency; reading the logits would take 1.4 of the 39 us.
 //
 // A CTA's 32 tokens leave one word per expert, a bit for every token that chose it (a token chooses an expert once).  A pair's row is what the words ahead count, and the
 // bits below its own: no order of arrival enters, so the rows are the same every time.  Up to 256 tokens: a cluster's CTAs read one another's words, one launch.
@@ -185,6 +187,22 @@ __device__ __noinline__ int exact_choice(const spk_route_scores_args& a, const T
     return mine;
 }
 
+// Falling order; a network of exchanges.
+template <int P>
+__device__ __forceinline__ void sort_keys(uint32_t (&key)[P]) {
+#pragma unroll
+    for (int k = 2; k <= P; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1)
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if ((i & j) == 0) {
+                    const uint32_t hi = max(key[i], key[i | j]), lo = min(key[i], key[i | j]);
+                    key[i] = (i & k) == 0 ? hi : lo;
+                    key[i | j] = (i & k) == 0 ? lo : hi;
+                }
+}
+
 // The token's choices.  x, b: this lane's logits and biases (expert lane + 32 i), bit: where a group's bit is, c64: 2 E doubles of shared memory of this warp.  A key's last bits name the
 // expert's place in the lane, the first of equal ones the largest.
 template <typename T, int P>
@@ -254,15 +272,13 @@ __device__ __forceinline__ int choose(const spk_route_scores_args& a, const T* l
     uint32_t key[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) key[i] = v[i] == -INFINITY ? 0u : (key_of(v[i]) & ~PLACE) | (PLACE - i);
+    sort_keys<P>(key);  // the lane's best is its first, and a choice moves its others up
     const float off = off_of(a.score, true, P > 8);
     int mine = -1, last = 0;
     float before = 0.0f, apart = 0.0f;
     bool settled = true;
     for (int j = 0; j <= a.top; ++j) {
-        uint32_t most = key[0];
-#pragma unroll
-        for (int i = 1; i < P; ++i) most = max(most, key[i]);
-        const uint32_t best = __reduce_max_sync(~0u, most);
+        const uint32_t most = key[0], best = __reduce_max_sync(~0u, most);
         if (best == 0) {
             before = -INFINITY;  // everything there is has been chosen
             break;
@@ -272,9 +288,11 @@ __device__ __forceinline__ int choose(const spk_route_scores_args& a, const T* l
         // experts of the very same logit and bias are equal in 64 bits too
         if (j > 0 && !(before - y > apart) && (logit(l, last) != logit(l, e) || (a.bias != nullptr && a.bias[last] != a.bias[e]))) settled = false;
         if (j == a.top) break;
+        if (lane == who) {
 #pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (i == place && lane == who) key[i] = 0;
+            for (int i = 0; i + 1 < P; ++i) key[i] = key[i + 1];
+            key[P - 1] = 0;
+        }
         if (lane == j) mine = e;
         before = y;
         apart = off * (fabsf(y) + bias_most) + kLeast;
@@ -352,9 +370,9 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
     }
     bias_most = warp_most(bias_most);
     int bit[P];
-    const int per = E / a.groups, L = a.groups <= 32 ? lanes_of(a.groups) : 1;
+    const int per = E / a.groups, L = a.groups <= 32 ? lanes_of(a.groups) : 1, inverse = ((1 << 20) + per - 1) / per;
 #pragma unroll
-    for (int i = 0; i < P; ++i) bit[i] = min(31, (lane + 32 * i) / per * L);
+    for (int i = 0; i < P; ++i) bit[i] = min(31, (lane + 32 * i) * inverse / (1 << 20) * L);  // expert / per: experts and groups of up to 1024
     __syncthreads();
     for (int i = warp; i < tokens; i += warps) {
         const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens + i;
@@ -480,7 +498,7 @@ int64_t words_of(int64_t n) { return (n + kTokens - 1) / kTokens; }
 
 template <typename T, int P, bool WHOLE>
 int launch_select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStream_t s) {
-    // a cluster of eight CTAs shares few tokens evenly (64 rows of 256 experts: XXX us, 19.4 as two CTAs of 32)
+    // a cluster of eight CTAs shares few tokens evenly: a CTA's warps share four schedulers (eight tokens each 9.5 us, 32 each 14.8)
     const int tokens = WHOLE ? static_cast<int>((a.n + kMostCluster - 1) / kMostCluster) : kTokens;
     if (WHOLE) n_words = static_cast<int>((a.n + tokens - 1) / tokens);
     // 64-bit scores of a warp are kept in shared memory: as many warps as fit
