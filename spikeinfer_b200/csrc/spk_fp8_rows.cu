@@ -331,6 +331,8 @@ bool stream_boundary8(const spk_rms_residual_fp8_args& p, cudaStream_t s, int* r
     constexpr int F = sizeof(TX) / 2;
     const int groups = static_cast<int>(p.width * sizeof(TX) / 16), stage = static_cast<int>(p.width * (sizeof(TX) + (p.delta != nullptr ? sizeof(TD) : 0)));
     if (p.pairs != nullptr || p.n < 592 || kStages * stage > 110 * 1024 || groups > (F == 1 ? 1024 : 128 * F)) return false;
+    // bulk copies: 16-byte boundaries (16-bit rows beside 32-bit ones of a multiple of four columns may have eight)
+    if (p.delta != nullptr && (p.width * sizeof(TD) % 16 != 0 || reinterpret_cast<uintptr_t>(p.delta) % 16 != 0)) return false;
     if (groups <= 128 * F) *rc = launch_stream<TX, TD, 2 * F, 64>(p, stage, s);
     else if constexpr (F == 1) *rc = groups <= 256 ? launch_stream<TX, TD, 1, 256>(p, stage, s) : groups <= 512 ? launch_stream<TX, TD, 2, 256>(p, stage, s) : launch_stream<TX, TD, 4, 256>(p, stage, s);
     return true;

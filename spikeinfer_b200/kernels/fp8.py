@@ -57,7 +57,7 @@ def rms_residual_fp8(x: torch.Tensor, weight: torch.Tensor, *, eps: float, delta
                      pairs: torch.Tensor | None = None, pair_slots: torch.Tensor | None = None, pair_weights: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """One layer boundary: ``y = x + delta + sum_j pair_weights[t, j] * pairs[pair_slots[t, j]]`` in the dtype of ``x``, to ``x_out`` (may be ``x``);
-    returns ``rmsnorm(y) * weight`` as e4m3 values and scales, and writes it to ``out`` (fp32 or bf16) where given.
+    returns ``rmsnorm(y) * weight`` as e4m3 values and scales, and writes it to ``out`` (fp32 or bf16) where given.  Up to 32768 columns.
 
     ``x`` is fp32 (``delta`` fp32 or bf16) or bf16 (``delta`` bf16), ``pairs`` what :func:`.experts.experts_forward` returned, ``pair_slots`` and
     ``pair_weights`` a route's (:func:`.routing.route_by_scores`); a negative slot adds nothing."""

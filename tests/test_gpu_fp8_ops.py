@@ -48,7 +48,7 @@ NORM = 16 * U
 
 @pytest.mark.parametrize("stream,delta_dtype", [(F32, F32), (F32, BF), (F32, None), (BF, BF), (BF, None)])
 @pytest.mark.parametrize("n,width,top", [(1, 1, 0), (1, 45, 1), (37, 88, 3), (5, 129, 0), (3, 896, 0), (2, 1022, 2), (64, 3584, 2), (7, 1028, 6), (3, 9001, 2),
-                                         (2, 32768, 1), (700, 256, 0), (601, 1030, 2)])
+                                         (2, 32768, 1), (700, 256, 0), (601, 1030, 2), (600, 900, 0), (593, 1004, 0), (640, 2056, 0)])
 def test_boundary(dev, n, width, top, stream, delta_dtype):
     g = gen(n * 7 + width)
     rnd = lambda *s: torch.randn(*s, generator=g)
@@ -86,6 +86,22 @@ def test_boundary(dev, n, width, top, stream, delta_dtype):
     q2, s2 = k8.rms_residual_fp8(d(x), d(w), eps=eps, delta=d(delta), status=status, **on)
     assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, scales)
     assert int(status.item()) == 0
+
+
+def test_boundary_of_matrices_at_odd_places(dev):
+    """Views that begin off every boundary but their own elements', many rows and few: the bits of aligned ones."""
+    for n, width in ((700, 512), (5, 512)):
+        for stream, delta_dtype in ((F32, F32), (F32, BF), (BF, BF)):
+            place = lambda t, off: torch.empty(t.numel() + off, dtype=t.dtype, device=dev)[off:].view(t.shape).copy_(t)
+            x, delta, w = torch.randn(n, width, device=dev).to(stream), torch.randn(n, width, device=dev).to(delta_dtype), torch.rand(width, device=dev)
+            run = lambda x, delta, w, x_out, out: (x_out, out, *k8.rms_residual_fp8(x, w, eps=1e-5, delta=delta, x_out=x_out, out=out))
+            want = run(x, delta, w, torch.empty_like(x), torch.empty(n, width, dtype=BF, device=dev))
+            for offs in ((1, 0, 0, 0, 0), (0, 1, 0, 0, 0), (0, 0, 1, 0, 0), (0, 0, 0, 1, 0), (0, 0, 0, 0, 1), (2, 2, 2, 2, 2), (4, 4, 4, 4, 4), (0, 4, 0, 0, 0)):
+                got = run(*(place(t, o) for t, o in zip((x, delta, w, want[0], want[1]), offs)))
+                v = fo.rms_norm(got[0].cpu(), w.cpu(), 1e-5)
+                assert torch.equal(got[0], want[0])
+                assert ((got[1].double().cpu() - v).abs() <= (NORM + HALF[BF]) * (1 + 2 * U) * v.abs()).all()
+                holds8(got[2], got[3], v, NORM)
 
 
 def test_boundary_reports_slots_that_do_not_exist(dev):
