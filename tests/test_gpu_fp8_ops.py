@@ -436,3 +436,25 @@ def test_refusals(dev):
                  lambda: ke.ExpertRouter([experts(top=2)()], 9)):
         with pytest.raises((ValueError, TypeError)):
             call()
+
+
+def test_rows_beyond_32_bit_offsets(dev):
+    n, width = 140_000, 16_384  # 2.3 billion elements
+    z = torch.randn(1000, width, device=dev).to(BF).repeat(n // 1000, 1)
+    z[-3:] = 2 * z[-3:] + 1
+    q, s = k8.quantize_fp8(z)
+    few, scales = k8.quantize_fp8(z[-3:])
+    assert torch.equal(q[-3:].view(torch.uint8), few.view(torch.uint8)) and torch.equal(s[:, -3:], scales)
+    w, delta = torch.rand(width, device=dev), z
+    x_out = torch.empty_like(z)
+    q, s = k8.rms_residual_fp8(z, w, eps=1e-5, delta=delta, x_out=x_out)
+    y = torch.empty(3, width, dtype=BF, device=dev)
+    few, scales = k8.rms_residual_fp8(z[-3:], w, eps=1e-5, delta=delta[-3:], x_out=y)
+    assert torch.equal(x_out[-3:], y)
+    holds8(q[-3:].clone(), s[:, -3:].clone(), fo.rms_norm(y.cpu(), w.cpu(), 1e-5), NORM)
+    holds8(few, scales, fo.rms_norm(y.cpu(), w.cpu(), 1e-5), NORM)
+    del z, q, x_out, delta
+    x, sx, w8, sw = operands(120_000, 256, 18_000, dev, 3)
+    out = k8.linear_fp8(x, sx, w8, sw)  # 2.16 billion elements
+    for at in (slice(119_900, 120_000), slice(0, 50)):
+        check_linear(out[at], x[at], sx[:, at], w8, sw)
