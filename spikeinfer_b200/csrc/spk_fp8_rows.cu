@@ -101,6 +101,18 @@ __device__ __forceinline__ void store_cols(T* p, const Cols<C>& r, int left) {
         spk_store4<float, true>(p + 4, make_float4(r.f[4], r.f[5], r.f[6], r.f[7]), left);
     }
 }
+// What the stream keeps of r: as it is in 32 bits, or rounded to bf16, pairs at a time (an element at a time the conversions filled the special-function unit to 29 %).
+template <int C, typename T>
+__device__ __forceinline__ void round_cols(Cols<C>& r) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < C; i += 2) {
+            const uint32_t u = pack_bf16(r.f[i], r.f[i + 1]);
+            r.f[i] = __uint_as_float(u << 16);
+            r.f[i + 1] = __uint_as_float(u & 0xffff0000u);
+        }
+    }
+}
 // First column of a thread's group, of those that begin at multiples of the block's threads.
 template <int C, int VEC>
 __device__ __forceinline__ int first_col(int thread) {
@@ -211,10 +223,7 @@ boundary8_kernel(const spk_rms_residual_fp8_args p) {
     float q[1] = {0.0f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        if (sizeof(TX) == 2) {  // the norm of what the next boundary will read
-#pragma unroll
-            for (int i = 0; i < C; ++i) y[v].f[i] = spk_to_float<TX>(spk_from_float<TX>(y[v].f[i]));
-        }
+        round_cols<C, TX>(y[v]);  // the norm of what the next boundary will read
         if (p.x_out != nullptr) store_cols<C, VEC>(static_cast<TX*>(p.x_out) + t * p.width + col(v), y[v], width - col(v));
 #pragma unroll
         for (int i = 0; i < C; i += 4)
@@ -283,10 +292,7 @@ boundary8_stream_kernel(const spk_rms_residual_fp8_args p) {
 #pragma unroll
                 for (int k = 0; k < C; ++k) y[v].f[k] += f.f[k];
             }
-            if (sizeof(TX) == 2) {
-#pragma unroll
-                for (int k = 0; k < C; ++k) y[v].f[k] = spk_to_float<TX>(spk_from_float<TX>(y[v].f[k]));
-            }
+            round_cols<C, TX>(y[v]);
             if (p.x_out != nullptr) store_cols<C, kWide>(static_cast<TX*>(p.x_out) + t * p.width + c, y[v], width - c);
 #pragma unroll
             for (int k = 0; k < C; k += 4)
@@ -364,7 +370,7 @@ int launch_boundary8(const spk_rms_residual_fp8_args& p, cudaStream_t s) {
 __device__ __forceinline__ float gelu_tanh(float z) { return z * rcp(1.0f + ex2(-2.302208198f * fmaf(0.044715f * z * z, z, z))); }  // 2 sqrt(2 / pi) log2(e)
 __device__ __forceinline__ float silu(float z) { return z * sigmoid_fast(z); }
 
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 128;  // 256: gate of 8192 x 18944 133 us against 128
 
 // A warp (C = 4) or half-warp (C = 8) takes U blocks of 128 columns that lie one after the other; all of their loads are under way together.
 template <typename T, int ACT, int VEC, int U>
@@ -404,7 +410,7 @@ int launch_quantize8(const spk_quantize_fp8_args& p, cudaStream_t s) {
     auto at = [&](int e) { return p.width % e == 0 && p.z_stride % e == 0 && reinterpret_cast<uintptr_t>(p.z) % (e * sizeof(T)) == 0; };
     constexpr int e = 16 / sizeof(T);
     const bool wide = at(e);
-    // One / two / four blocks at a time, us: 37 x 4864 bf16 gelu 1.85 / 2.11 / 2.96, 512 rows 4.6 / 4.3 / 5.1, 8192 rows 40.4 / 36.4 / 35.3; 8192 x 18944 gate 149 / 132 / 127, without activation
+    // One / two / four blocks at a time, us: 37 x 4864 bf16 gelu 1.85 / 2.11 / 2.96, 512 rows 4.6 / 4.3 / 5.1, 8192 rows 40.4 / 36.4 / 35.3; 8192 x 18944 gate 149 / 132 / 127 (with 256 threads a CTA), without activation
     // 103 / 89 / 92.
     constexpr int U4 = ACT != SPK_ACT_NONE && sizeof(T) == 2 ? 4 : 2;
     const int u = blocks < 16384 ? 1 : wide && blocks >= 262144 ? U4 : 2, per = kQuantThreads / (wide ? 128 / e : 32) * u;

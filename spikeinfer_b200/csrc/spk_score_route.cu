@@ -456,26 +456,32 @@ score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ 
     extern __shared__ int32_t sm32[];  // [experts] twice, 32
     const int E = a.experts, w0 = blockIdx.x * kLayoutWords, row = (n_words + 3) & ~3, quads = row / 4;
     int32_t *at = sm32, *before = at + E;
-    for (int e = threadIdx.x; e < 2 * E; e += kLayoutThreads) sm32[e] = 0;
-    __syncthreads();
     spk_grid_wait();
     auto load = [&](int e, int q) { return __ldcg(reinterpret_cast<const uint4*>(words + static_cast<int64_t>(e) * row) + q); };
     auto count = [](const uint4& u, int n) {  // of the first n words
         return (n > 0 ? __popc(u.x) : 0) + (n > 1 ? __popc(u.y) : 0) + (n > 2 ? __popc(u.z) : 0) + (n > 3 ? __popc(u.w) : 0);
     };
-    // lanes side by side take a row's words, 16 bytes each: 16 loads of 1024 threads bring 8192 tokens' words of 256 experts
-    const int side = quads < 32 ? quads < 4 ? 1 : quads < 16 ? 4 : 16 : 32;
-    for (int e = threadIdx.x / side; e < E; e += kLayoutThreads / side) {
+    // Lanes side by side take a row's words, 16 bytes each and about eight loads a lane: 8192 tokens' words of 256 experts in two passes.
+    int side = 1;
+    while (side < 32 && 8 * side < quads) side <<= 1;
+    for (int e0 = 0; e0 < E; e0 += kLayoutThreads / side) {
+        const int e = e0 + threadIdx.x / side;
         int all = 0, ahead = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int q = threadIdx.x % side; q < quads; q += side) {
-            const uint4 u = load(e, q);
-            const int c = count(u, 4);
+            const int c = e < E ? count(load(e, q), 4) : 0;
             all += c;
             if (4 * q < w0) ahead += c;  // w0 is a multiple of four
         }
-        if (all != 0) atomicAdd(at + e, all);
-        if (ahead != 0) atomicAdd(before + e, ahead);
+        __syncwarp();
+        for (int o = side >> 1; o >= 1; o >>= 1) {
+            all += __shfl_xor_sync(~0u, all, o);
+            ahead += __shfl_xor_sync(~0u, ahead, o);
+        }
+        if (e < E && threadIdx.x % side == 0) {
+            at[e] = all;
+            before[e] = ahead;
+        }
     }
     __syncthreads();
     lay_out(a, blockIdx.x == 0, at, before, before + E);
