@@ -3,12 +3,12 @@
 // A warp per token, an expert of every 32 per lane.  Choices lie next to borders, where 32 bits would tell equal from unequal by how they were rounded, so they have to
 // come out as in 64-bit arithmetic.  Nearly all of them are settled by 32-bit scores: where every difference that decides (each choice from the next, the worst group kept from
 // the best one dropped) is beyond what the scores can be off by, it has the sign of the exact one.  Where one is not, the groups, or the experts that can be among the chosen, are
-// compared in 64 bits.  (64 bits for every token: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44; for the whole of a token that is not settled: 49 and 13; so 39 and 9.5.)
+// compared in 64 bits.  (64 bits for every token: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44; for the whole of a token that is not settled: 49 and 13; so, with the layout's loads side by side, 34 and 9.5.)
 //
-// What bounds it: some 1300 instructions a token (scores 200, groups 250, choices 500, weights 100) and their latency; reading the logits would take 1.4 of the 39 us.
+// What bounds it: some 1300 instructions a token (scores 200, groups 250, choices 500, weights 100) and their latency; reading the logits would take 1.4 of the 34 us.
 //
 // A CTA's 32 tokens leave one word per expert, a bit for every token that chose it (a token chooses an expert once).  A pair's row is what the words ahead count, and the
-// bits below its own: no order of arrival enters, so the rows are the same every time.  Up to 256 tokens: a cluster's CTAs read one another's words, one launch.
+// bits below its own: no order of arrival enters, so the rows are the same every time.  Up to 128 tokens: a cluster's CTAs read one another's words, one launch.
 // More: score_layout_kernel, from the words in memory.
 #include "spk_experts.cuh"
 #include "spk_tensor.cuh"
@@ -19,6 +19,7 @@ using namespace spk_tc;
 
 constexpr int kTokens = 32;        // per CTA of the selection, at most: the bits of a word
 constexpr int kMostCluster = 8;    // CTAs that hand out the rows among themselves
+constexpr int kMostWhole = 128;    // tokens of such a launch
 constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutWords = 8;    // words per CTA of the layout
 
@@ -452,7 +453,7 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
 }
 
 __global__ void __launch_bounds__(kLayoutThreads)
-score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ words, const int n_words) {
+score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ words, const int n_words, const int tokens) {
     extern __shared__ int32_t sm32[];  // [experts] twice, 32
     const int E = a.experts, w0 = blockIdx.x * kLayoutWords, row = (n_words + 3) & ~3, quads = row / 4;
     int32_t *at = sm32, *before = at + E;
@@ -485,31 +486,32 @@ score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ 
     }
     __syncthreads();
     lay_out(a, blockIdx.x == 0, at, before, before + E);
-    const int64_t lo = static_cast<int64_t>(w0) * kTokens * a.top;
-    const int pairs = static_cast<int>(min(static_cast<int64_t>(kLayoutWords) * kTokens, a.n - static_cast<int64_t>(w0) * kTokens)) * a.top;
+    const int64_t lo = static_cast<int64_t>(w0) * tokens * a.top;
+    const int pairs = static_cast<int>(min(static_cast<int64_t>(kLayoutWords) * tokens, a.n - static_cast<int64_t>(w0) * tokens)) * a.top;
     for (int i = threadIdx.x; i < pairs; i += kLayoutThreads) {
         const int e = __ldcg(a.ids + lo + i);
         int slot = -1;
         if (e >= 0) {
-            const int t = i / a.top, w = t / kTokens;  // word of the CTA's
+            const int t = i / a.top, w = t / tokens;  // word of the CTA's
             const uint4 u = load(e, w0 / 4), v = w0 / 4 + 1 < quads ? load(e, w0 / 4 + 1) : make_uint4(0u, 0u, 0u, 0u);
             const uint32_t own = w < 4 ? (w < 2 ? (w == 0 ? u.x : u.y) : (w == 2 ? u.z : u.w)) : (w < 6 ? (w == 4 ? v.x : v.y) : (w == 6 ? v.z : v.w));
-            slot = before[e] + __popc(own & ((1u << (t % kTokens)) - 1u)) + count(u, w) + count(v, w - 4);
+            slot = before[e] + __popc(own & ((1u << (t % tokens)) - 1u)) + count(u, w) + count(v, w - 4);
         }
         a.slots[lo + i] = slot;
     }
 }
 
-int64_t words_of(int64_t n) { return (n + kTokens - 1) / kTokens; }
+// Tokens per CTA of the selection.  Up to 128 in all: eight CTAs share them evenly (a CTA's warps share four schedulers: 64 rows of 256 experts 9.5 us, 256 rows 14.9).  More: eight each while all of
+// them are on the chip at once (257 and 1024 rows 12.9 and 14.5 us, with 32 each 19.9 and 22.5).
+int tokens_of(int64_t n) { return n <= kMostWhole ? static_cast<int>((n + kMostCluster - 1) / kMostCluster) : n <= 148 * 8 ? 8 : n <= 148 * 16 ? 16 : kTokens; }
+int64_t words_of(int64_t n) { return n < 1 ? 0 : (n + tokens_of(n) - 1) / tokens_of(n); }
 
 template <typename T, int P, bool WHOLE>
 int launch_select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStream_t s) {
-    // a cluster of eight CTAs shares few tokens evenly: a CTA's warps share four schedulers (eight tokens each 9.5 us, 32 each 14.8)
-    const int tokens = WHOLE ? static_cast<int>((a.n + kMostCluster - 1) / kMostCluster) : kTokens;
-    if (WHOLE) n_words = static_cast<int>((a.n + tokens - 1) / tokens);
+    const int tokens = tokens_of(a.n);
     // 64-bit scores of a warp are kept in shared memory: as many warps as fit
     const int per = 16 * a.experts, extra = 4 * a.experts + (WHOLE ? 4 * (kTokens * a.top + 2 * a.experts + 32) : 0);
-    int warps = !WHOLE ? 16 : tokens < 8 ? 8 : tokens;  // eight at least hand out the rows
+    int warps = !WHOLE ? min(tokens, 16) : tokens < 8 ? 8 : tokens;  // eight at least hand out the rows
     while (warps * per + extra > 200 * 1024) warps /= 2;
     const int bytes = warps * per + extra;
     auto kernel = score_select_kernel<T, P, WHOLE>;
@@ -544,7 +546,7 @@ int select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStr
 }  // namespace
 
 extern "C" int64_t spk_route_scores_workspace_bytes(int64_t n, int experts) {
-    if (n <= kMostCluster * kTokens || experts < 1) return 0;
+    if (n <= kMostWhole || experts < 1) return 0;
     return (words_of(n) + 3) / 4 * 16 * experts;
 }
 
@@ -565,12 +567,12 @@ extern "C" int spk_route_scores(const spk_route_scores_args* args, void* stream)
     if (a.n > 0) {
         if (a.logits == nullptr || a.ids == nullptr || a.weights == nullptr || a.slots == nullptr) return SPK_ERR_NULL_POINTER;
         if (a.logits_stride < a.experts) return SPK_ERR_BAD_STRIDE;
-        if (n_words <= kMostCluster) return a.dtype == SPK_F32 ? select<float, true>(a, words, n_words, s) : select<__nv_bfloat16, true>(a, words, n_words, s);
+        if (a.n <= kMostWhole) return a.dtype == SPK_F32 ? select<float, true>(a, words, n_words, s) : select<__nv_bfloat16, true>(a, words, n_words, s);
         if (a.workspace == nullptr || a.workspace_bytes < spk_route_scores_workspace_bytes(a.n, a.experts)) return SPK_ERR_WORKSPACE_TOO_SMALL;
         if (reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) return SPK_ERR_BAD_STRIDE;
         const int rc = a.dtype == SPK_F32 ? select<float, false>(a, words, n_words, s) : select<__nv_bfloat16, false>(a, words, n_words, s);
         if (rc != SPK_OK) return rc;
     }
     const int grid = n_words == 0 ? 1 : (n_words + kLayoutWords - 1) / kLayoutWords;
-    return spk_launch(score_layout_kernel, dim3(grid), kLayoutThreads, sizeof(int32_t) * (2 * a.experts + 32), s, n_words > 0, a, words, n_words);
+    return spk_launch(score_layout_kernel, dim3(grid), kLayoutThreads, sizeof(int32_t) * (2 * a.experts + 32), s, n_words > 0, a, words, n_words, tokens_of(a.n));
 }

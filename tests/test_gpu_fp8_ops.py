@@ -252,7 +252,7 @@ def check_route(r, logits, top, **kw):
 
 
 ROUTES = [(1, 16, 2, 1, 1), (1, 1, 1, 1, 1), (3, 5, 5, 1, 1), (64, 256, 8, 8, 4), (33, 60, 4, 1, 1), (257, 64, 6, 8, 3), (40, 160, 6, 8, 3), (9, 384, 8, 1, 1), (7, 1024, 32, 1, 1),
-          (5, 1024, 16, 32, 2), (300, 8, 2, 4, 2), (31, 12, 2, 12, 5), (65, 100, 7, 4, 2), (1000, 37, 3, 1, 1)]
+          (5, 1024, 16, 32, 2), (300, 8, 2, 4, 2), (31, 12, 2, 12, 5), (65, 100, 7, 4, 2), (1000, 37, 3, 1, 1), (2000, 24, 2, 1, 1)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
