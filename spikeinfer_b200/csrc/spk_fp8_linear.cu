@@ -24,8 +24,8 @@ using namespace spk_tc;
 
 constexpr int kBlock = 128;              // columns with a scale, and bytes of a tile's row
 constexpr int kTileW = kBlock * kBlock;  // bytes of a weight tile: 128 features
-constexpr int kGroup = 8;  // tiles: blocks of k whose scales come together
-constexpr int kGroups = 4;
+constexpr int kGroup = 8;                // tiles: blocks of k whose scales come together
+constexpr int kGroups = 4;               // of those in the ring
 
 // Few rows: blocks of k come in groups of kRun, each with accumulators of its own and one barrier for the group (1.3 us a block of 64 tokens with one each).
 constexpr int kRun = 4;
@@ -297,7 +297,7 @@ constexpr int kTileThreads = 128 + 32 * kWriters;
 // The scales of `kn` blocks of k, ROWS tokens and FB runs of 128 features, into a ring [kGroups][kGroup][ROWS + 4] (tokens, then runs), kGroup blocks at a time, by two
 // warps in turn with asynchronous copies.  Asked for one or two blocks ahead by the threads that use them, scales were waited for (1171 x 4864 x 896: 0.62 us a block, the
 // latency of HBM over two); a barrier for every block took 0.1 us of the 0.5 that a block of 128 x 256 took, and so did copies of four bytes where rows of scales are
-// aligned to 16 (`vec`).  g: groups so far; x: the first token's scale, of `rows` that exist; w: the first run's, of `runs`.  false where a wait ran out.
+// aligned to 16 (`vec`).  g: groups so far; x: the first token's scale, of `rows` that exist (none: any scale); w: the first run's, of `runs`.  false where a wait ran out.
 template <int ROWS, int FB>
 __device__ __forceinline__ bool bring_scales(Bars* bars, float* ring, int who, int& g, int kn, const float* x, int64_t x_step, int rows, int vec, const float* w, int64_t w_run, int runs,
                                              volatile int* abort) {
@@ -339,6 +339,7 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// On a barrier of any CTA of the cluster.  What is handed over is tensor memory, ordered by the tcgen05 fences: no release of cluster scope, which took some 2 us.
 __device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -451,70 +452,73 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
     auto m_of = [&](int tile) { return tile / per_panel * kPanel + tile % per_panel % high(tile); };
     auto n_of = [&](int tile) { return tile % per_panel / high(tile); };
     if (warp < 4) {  // 128 x 56 + 256 x 224 registers: the launch's 384 x 168
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      if (warp == 0) {
-        if (lane == 0) {
-            int c = 0;
-            bool go = true;
-            for (int tile = first; tile < tiles && go; tile += stride) {
-                const int t0 = m_of(tile) * 128 * CG + rank * 128, f0 = n_of(tile) * NF + rank * Sh::kRowsW;
-                for (int k = 0; k < kn; ++k, ++c) {
-                    const int s = c % NS;
-                    if (c >= NS && !mbar_wait(smem_u32(&bars->free[s]), ((c / NS) - 1) & 1, abort)) {
-                        go = false;
-                        break;
-                    }
-                    const uint32_t dst = smem_u32(base + s * Sh::kStage);
-                    if (CG == 1) {
-                        const uint32_t bar = smem_u32(&bars->full[s]);
-                        mbar_expect(bar, Sh::kStage);
-                        tma_load(dst, &x_map, (kb + k) * kBlock, t0, bar);
-                        tma_load(dst + kTileW, &w_map, (kb + k) * kBlock, f0, bar);
-                    } else {
-                        const uint32_t bar = at_rank(smem_u32(&bars->full[s]), 0);
-                        if (rank == 0) mbar_expect(smem_u32(&bars->full[s]), 2 * Sh::kStage);
-                        tma_load_pair(dst, &x_map, (kb + k) * kBlock, t0, bar);
-                        tma_load_pair(dst + kTileW, &w_map, (kb + k) * kBlock, f0, bar);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            if (lane == 0) {
+                int c = 0;
+                bool go = true;
+                for (int tile = first; tile < tiles && go; tile += stride) {
+                    const int t0 = m_of(tile) * 128 * CG + rank * 128, f0 = n_of(tile) * NF + rank * Sh::kRowsW;
+                    for (int k = 0; k < kn; ++k, ++c) {
+                        const int s = c % NS;
+                        if (c >= NS && !mbar_wait(smem_u32(&bars->free[s]), ((c / NS) - 1) & 1, abort)) {
+                            go = false;
+                            break;
+                        }
+                        const uint32_t dst = smem_u32(base + s * Sh::kStage);
+                        if (CG == 1) {
+                            const uint32_t bar = smem_u32(&bars->full[s]);
+                            mbar_expect(bar, Sh::kStage);
+                            tma_load(dst, &x_map, (kb + k) * kBlock, t0, bar);
+                            tma_load(dst + kTileW, &w_map, (kb + k) * kBlock, f0, bar);
+                        } else {
+                            const uint32_t bar = at_rank(smem_u32(&bars->full[s]), 0);
+                            if (rank == 0) mbar_expect(smem_u32(&bars->full[s]), 2 * Sh::kStage);
+                            tma_load_pair(dst, &x_map, (kb + k) * kBlock, t0, bar);
+                            tma_load_pair(dst + kTileW, &w_map, (kb + k) * kBlock, f0, bar);
+                        }
                     }
                 }
+                // copies in flight land before the CTA's shared memory is given up
+                if (*abort != 0 && rank == 0)
+                    for (int k = c > NS ? c - NS : 0; k < c; ++k) mbar_wait(smem_u32(&bars->full[k % NS]), (k / NS) & 1);
             }
-            // copies in flight land before the CTA's shared memory is given up
-            if (*abort != 0 && rank == 0)
-                for (int k = c > NS ? c - NS : 0; k < c; ++k) mbar_wait(smem_u32(&bars->full[k % NS]), (k / NS) & 1);
-        }
-      } else if (warp == 1) {
-        if (rank == 0) {  // in code that the whole warp runs: descriptors stay in uniform registers
-            constexpr uint32_t idesc = idesc_e4m3(128 * CG, NF);
-            const uint32_t who = elect_one();
-            int c = 0;
-            bool go = true;
-            for (int tile = first; tile < tiles && go; tile += stride) {
-                for (int k = 0; k < kn; ++k, ++c) {
-                    const int s = c % NS, b = c % NB;
-                    go = __all_sync(~0u, (c < NB || mbar_wait(smem_u32(&bars->drained[b]), ((c / NB) - 1) & 1, abort)) &&
-                                             mbar_wait(smem_u32(&bars->full[s]), (c / NS) & 1, abort));
-                    if (!go) break;
-                    tc_fence_after();
-                    const uint32_t xa = smem_u32(base + s * Sh::kStage), wa = xa + kTileW;
+        } else if (warp == 1) {
+            if (rank == 0) {  // in code that the whole warp runs: descriptors stay in uniform registers
+                constexpr uint32_t idesc = idesc_e4m3(128 * CG, NF);
+                const uint32_t who = elect_one();
+                int c = 0;
+                bool go = true;
+                for (int tile = first; tile < tiles && go; tile += stride) {
+                    for (int k = 0; k < kn; ++k, ++c) {
+                        const int s = c % NS, b = c % NB;
+                        go = __all_sync(~0u, (c < NB || mbar_wait(smem_u32(&bars->drained[b]), ((c / NB) - 1) & 1, abort)) &&
+                                                 mbar_wait(smem_u32(&bars->full[s]), (c / NS) & 1, abort));
+                        if (!go) break;
+                        tc_fence_after();
+                        const uint32_t xa = smem_u32(base + s * Sh::kStage), wa = xa + kTileW;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma_e4m3_by<CG>(who, tmem + b * NF, desc_sw128(xa + i * 32, 16, 1024), desc_sw128(wa + i * 32, 16, 1024), idesc, i > 0);
-                    commit_by<CG>(who, smem_u32(&bars->free[s]));
-                    commit_by<CG>(who, smem_u32(&bars->sums[b]));
+                        for (int i = 0; i < 4; ++i) mma_e4m3_by<CG>(who, tmem + b * NF, desc_sw128(xa + i * 32, 16, 1024), desc_sw128(wa + i * 32, 16, 1024), idesc, i > 0);
+                        commit_by<CG>(who, smem_u32(&bars->free[s]));
+                        commit_by<CG>(who, smem_u32(&bars->sums[b]));
+                    }
                 }
+                commit_by<CG>(who, smem_u32(&bars->done));
+                mbar_wait(smem_u32(&bars->done), 0);  // nothing this warp issued is in the tensor pipe any more
+            } else {
+                mbar_wait(smem_u32(&bars->done), 0);  // the even CTA's arrivals here have all been made
             }
-            commit_by<CG>(who, smem_u32(&bars->done));
-            mbar_wait(smem_u32(&bars->done), 0);  // nothing this warp issued is in the tensor pipe any more
+        } else {
+            int g = 0;
+            for (int tile = first; tile < tiles; tile += stride) {
+                const int64_t t = static_cast<int64_t>(m_of(tile)) * 128 * CG + rank * 128, fb = static_cast<int64_t>(n_of(tile)) * FB;
+                if (!bring_scales<128, FB>(bars, ring, warp - 2, g, kn, a.x_scales + kb * a.x_scale_stride + (t < a.n ? t : 0), a.x_scale_stride,
+                                           static_cast<int>(max(min(a.n - t, static_cast<int64_t>(128)), static_cast<int64_t>(0))), vec_scales,
+                                           a.w_scales + fb * a.w_scale_stride + kb, a.w_scale_stride, static_cast<int>(min((a.features + 127) / 128 - fb, static_cast<int64_t>(FB))), abort))
+                    break;
+            }
+            cp_async_wait_all();
         }
-      } else {
-        int g = 0;
-        for (int tile = first; tile < tiles; tile += stride) {
-            const int64_t t = static_cast<int64_t>(m_of(tile)) * 128 * CG + rank * 128, fb = static_cast<int64_t>(n_of(tile)) * FB;
-            if (!bring_scales<128, FB>(bars, ring, warp - 2, g, kn, a.x_scales + kb * a.x_scale_stride + t, a.x_scale_stride, static_cast<int>(min(a.n - t, static_cast<int64_t>(128))), vec_scales,
-                                       a.w_scales + fb * a.w_scale_stride + kb, a.w_scale_stride, static_cast<int>(min((a.features + 127) / 128 - fb, static_cast<int64_t>(FB))), abort))
-                break;
-        }
-        cp_async_wait_all();
-      }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quad = warp & 3, half = (warp - 4) / 4, r = quad * 32 + lane;
