@@ -2,7 +2,8 @@
 
 Activations are e4m3 ``[n, width]`` with fp32 scales ``[ceil(width / 128), n]``, one for every row and 128 columns; weights are e4m3 ``[features, k]`` with
 fp32 scales ``[ceil(features / 128), ceil(k / 128)]``, one for every block of 128 x 128.  A value stands for ``value * scale``.  Rows start on
-16-byte boundaries: a width that is no multiple of 16 is a view of a wider matrix (:func:`rows_fp8`)."""
+16-byte boundaries: a width that is no multiple of 16 is a view of a wider matrix (:func:`rows_fp8`).  The kernels are in the full library
+(``python -m spikeinfer_b200.build``), not in those that serve one model from a fresh checkout."""
 from __future__ import annotations
 
 import torch
@@ -40,6 +41,7 @@ def one_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
             raise ValueError(f"all tensors must be on {device}: one is on {t.device}")
 
 
+@torch.no_grad()
 def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """A weight matrix ``[features, k]`` as e4m3 values and scales for blocks of 128 x 128, for :func:`linear_fp8`; done once, when a model is loaded."""
     f, k = w.shape
