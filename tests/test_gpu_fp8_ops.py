@@ -411,6 +411,25 @@ def test_a_captured_block_and_one_beside_it(dev):
     assert int(status.item()) == 0 and keep
 
 
+def test_two_streams_of_products_and_routes(dev):
+    """Every form of the product, and routes of both, on two streams at once: the bits of one after the other."""
+    sizes = [(2600, 260, 4000), (5, 2100, 300), (90, 2304, 1100), (200, 2048, 1000), (64, 2050, 900), (2600, 260, 4000)]
+    work = [operands(*z, dev, i) for i, z in enumerate(sizes)]
+    logits = [torch.randn(n, 64, generator=torch.Generator(device=dev).manual_seed(n), device=dev) for n in (60, 700, 3000)]
+    run = lambda: [k8.linear_fp8(*w) for w in work] + [t for l in logits for r in (kr.route_by_scores(l, 4),) for t in (r.ids, r.weights, r.slots, r.segs)]
+    want = run()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(run())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
 # ---- refusals --------------------------------------------------------------------------------------------------------
 def test_refusals(dev):
     x, w = torch.randn(4, 48, device=dev), torch.ones(48, device=dev)
