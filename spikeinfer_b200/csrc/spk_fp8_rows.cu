@@ -330,8 +330,8 @@ int launch_stream(const spk_rms_residual_fp8_args& p, int stage, cudaStream_t s)
     return SPK_OK;
 }
 
-// Whether a batch goes to the streaming form, and its launch: no expert rows, enough rows, and 16-bit or narrow ones (8192 rows, the form above / streaming, us: 3584 bf16 57 / 40, 896 bf16
-// 17.0 / 12.7, 896 fp32 22.9 / 20.6, 3584 fp32 68 / 72).  Narrow rows have two warps each (one 14.3 and 27.1, four 14.4 and 23.4).
+// Whether a batch goes to the streaming form, and its launch: no expert rows, enough rows, and 16-bit or narrow ones (8192 rows, the form above / streaming, us: 3584 bf16 106 / 37, 896 bf16
+// 17.0 / 11.8, 896 fp32 22.9 / 20.5, 3584 fp32 61 / 72).  Narrow rows have two warps each (one 14.3 and 27.1, four 14.4 and 23.4).
 template <typename TX, typename TD>
 bool stream_boundary8(const spk_rms_residual_fp8_args& p, cudaStream_t s, int* rc) {
     constexpr int F = sizeof(TX) / 2;
