@@ -1,0 +1,62 @@
+"""GPU: the 8-bit operators and the routes by scores where their contract says more than a tolerance."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import fp8_oracle as fo
+from spikeinfer_b200.kernels import fp8 as k8
+
+from test_gpu_fp8_ops import BF, F32, FP8, gen
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- the 8-bit value and its scale ----------------------------------------------------------------------------------
+def is_quotient(q, scales, v):
+    """scales are most / 448 and q is v / scale to the nearest, both as 32-bit divisions round them: no other value, at a tie neither."""
+    v = v.float().cpu()
+    n, width = v.shape
+    blocks = -(-width // 128)
+    padded = torch.zeros(n, blocks * 128)
+    padded[:, :width] = v
+    padded = padded.view(n, blocks, 128)
+    most = torch.where(padded.isnan(), 0.0, padded.abs()).clamp(max=torch.finfo(F32).max).amax(2).clamp(min=fo.LEAST)
+    want = most / 448.0
+    assert torch.equal(scales.cpu(), want.t())
+    values = (padded / want[..., None]).clamp(-448.0, 448.0).to(FP8).view(n, -1)[:, :width]
+    assert torch.equal(torch.nan_to_num(q.cpu().float(), nan=-1000.0), torch.nan_to_num(values.float(), nan=-1000.0))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n,width,pad", [(37, 4864, 0), (300, 1021, 1), (300, 1022, 2), (3000, 896, 0), (3000, 898, 0), (2500, 897, 0), (8192, 4864, 0)])
+def test_values_are_the_nearest_to_the_quotient(dev, n, width, pad, dtype):
+    """16-bit values over a scale of few bits lie between two 8-bit ones often (one in a thousand): the even one is theirs."""
+    z = torch.full((n, width + pad), float("nan"), dtype=dtype, device=dev)[:, pad // 2: pad // 2 + width]
+    z.copy_(torch.randn(n, width, generator=torch.Generator(device=dev).manual_seed(n + width), device=dev))
+    if dtype == F32:
+        z.mul_(2.0 ** torch.randint(-90, 100, (n, 1), generator=torch.Generator(device=dev).manual_seed(1), device=dev))
+    q, scales = k8.quantize_fp8(z)
+    is_quotient(q, scales, z)
+
+
+@pytest.mark.parametrize("stream", [F32, BF])
+@pytest.mark.parametrize("n,width", [(5, 512), (3, 1022), (7, 1021), (64, 3584), (700, 256), (2000, 3584), (1300, 1030)])
+def test_boundary_rounds_what_it_writes(dev, n, width, stream):
+    g = torch.Generator(device=dev).manual_seed(n + width)
+    x, delta = (torch.randn(n, width, generator=g, device=dev).to(stream) for _ in range(2))
+    out = torch.empty(n, width, device=dev)
+    q, scales = k8.rms_residual_fp8(x, 1 + 0.2 * torch.randn(width, generator=g, device=dev), eps=1e-5, delta=delta, out=out)
+    is_quotient(q, scales, out)
+
+
+def test_quotients_of_values_that_are_not_finite(dev):
+    inf, nan = float("inf"), float("nan")
+    top = torch.finfo(F32).max
+    for dtype in (F32, BF):
+        for width in (512, 514, 513):
+            z = torch.randn(6, width, generator=gen(width)) * torch.tensor([1.0, 1e-30, 1e30, 1e-32, 1.0, 1.0])[:, None]
+            z[0, 3], z[0, 200], z[2, 5], z[2, 300], z[4, 7], z[5] = nan, inf, -inf, top, -top, 0.0
+            z = z.to(dtype)
+            q, scales = k8.quantize_fp8(z.to(dev))
+            is_quotient(q, scales, z)
