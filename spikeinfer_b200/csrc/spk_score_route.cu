@@ -287,7 +287,18 @@ __device__ __forceinline__ int choose(const spk_route_scores_args& a, const T* l
         const int who = __ffs(__ballot_sync(~0u, most == best)) - 1, place = PLACE - static_cast<int>(best & PLACE), e = who + 32 * place;  // equal ones by index
         const float y = of_key(best & ~PLACE);
         // experts of the very same logit and bias are equal in 64 bits too
-        if (j > 0 && !(before - y > apart) && (logit(l, last) != logit(l, e) || (a.bias != nullptr && a.bias[last] != a.bias[e]))) settled = false;
+        if (j > 0 && !(before - y > apart)) {
+            const float x0 = logit(l, last), b0 = a.bias != nullptr ? a.bias[last] : 0.0f;
+            if (x0 != logit(l, e) || (a.bias != nullptr && b0 != a.bias[e])) {
+                settled = false;
+            } else if (j == a.top && settled) {  // nor may one behind the cut, which is neither of the two, be better than they
+                bool other = false;
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    other = other || (v[i] != -INFINITY && (key_of(v[i]) & ~PLACE) <= key_of(before) && !(v[i] < before - apart) && (x[i] != x0 || b[i] != b0));
+                if (__any_sync(~0u, other)) settled = false;
+            }
+        }
         if (j == a.top) break;
         if (lane == who) {
 #pragma unroll

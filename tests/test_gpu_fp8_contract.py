@@ -6,8 +6,9 @@ import torch
 
 from oracle import fp8_oracle as fo
 from spikeinfer_b200.kernels import fp8 as k8
+from spikeinfer_b200.kernels import routing as kr
 
-from test_gpu_fp8_ops import BF, F32, FP8, gen
+from test_gpu_fp8_ops import BF, F32, FP8, check_route, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +61,47 @@ def test_quotients_of_values_that_are_not_finite(dev):
             z = z.to(dtype)
             q, scales = k8.quantize_fp8(z.to(dev))
             is_quotient(q, scales, z)
+
+
+# ---- choices ---------------------------------------------------------------------------------------------------------
+def rows_of(*rows, experts=12):
+    """Rows of logits; where a row is short, experts behind it that can't be chosen."""
+    out = torch.full((len(rows), experts), -float("inf"))
+    for r, row in zip(out, rows):
+        r[: len(row)] = torch.tensor(row)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("times", [1, 70])
+def test_equal_experts_at_the_cut_hide_none_behind_them(dev, times, dtype):
+    """The last of the chosen equals the next one, and one behind both that 32 bits cannot tell from them is better."""
+    sigmoid = rows_of([17, 17, 40, 0], [20, 20, 20, 25, 0, 0, 0, 0], [30, 30, 30, 30, 30, 30, 30, 31, 33, 35, 36, 36], [17, 17, 17, 40], [-200, -200, -100], [-120, -120, -120, -119, -120])
+    softmax = rows_of([0, -200, -200, -100], [0, -150, -150, -150, -150, -149], [0, -120, -120, -120, -110, -115], [5, 5, -300, -300, -299])
+    flat = rows_of([-20, -20, -19, -50], [-22, -22, -22, -22, -21], [-18, -18, -18, -17, -17])  # beside a bias that is 1 for all
+    one = torch.ones(12)
+    for logits, score, bias in ((sigmoid, "sigmoid", None), (softmax, "softmax", None), (flat, "sigmoid", one), (rows_of([0, -22, -22, -21], [0, -30, -30, -30, -29]), "softmax", one)):
+        logits = logits.repeat(times, 1).to(dtype)
+        for top in (1, 2, 3, 4, 8):
+            for groups, top_groups in ((1, 1), (3, 2)):
+                if top <= 12 // groups * top_groups:
+                    more = dict(score=score, bias=None if bias is None else bias.to(dev), groups=groups, top_groups=top_groups)
+                    check_route(kr.route_by_scores(logits.to(dev), top, **more), logits, top, **more)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,top", [(16, 2), (64, 6), (200, 1), (256, 8), (300, 4), (700, 5)])
+def test_choices_among_few_and_saturated_logits(dev, experts, top, score):
+    """Logits of a few values: ties at every cut, saturated ones among them, single better experts far behind."""
+    g = gen(experts)
+    values = torch.tensor([17.0, 17.5, 20.0, 30.0, 36.0, 40.0, -100.0, -200.0])
+    logits = values[torch.randint(0, 8, (40, experts), generator=g)]
+    logits[:20] = 20.0
+    logits[torch.arange(10), torch.randint(0, experts, (10,), generator=g)] = 25.0
+    logits[20:30] = torch.where(torch.rand(10, experts, generator=g) < 0.9, 17.0, logits[20:30])
+    logits[10] = 0.0
+    logits[11] = 0.0
+    logits[11, experts - 1] = 1e-9
+    for bias in (None, torch.full((experts,), 2.0)):
+        more = dict(score=score, bias=None if bias is None else bias.to(dev))
+        check_route(kr.route_by_scores(logits.to(dev), top, **more), logits, top, **more)
