@@ -505,8 +505,6 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
                 }
                 commit_by<CG>(who, smem_u32(&bars->done));
                 mbar_wait(smem_u32(&bars->done), 0);  // nothing this warp issued is in the tensor pipe any more
-            } else {
-                mbar_wait(smem_u32(&bars->done), 0);  // the even CTA's arrivals here have all been made
             }
         } else {
             int g = 0;
@@ -598,6 +596,8 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
         cluster_arrive();
         cluster_wait();  // no CTA leaves while its sums are being read, or its partner works in its memory
     }
+    // Behind the pair's barrier the even CTA has seen its last commit, so its arrivals here are all but made, however long the product took (a wait's limit is meant for one phase).
+    if (CG == 2 && rank != 0 && warp == 1 && !mbar_wait(smem_u32(&bars->done), 0)) *abort = 1;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -8,7 +8,7 @@ from oracle import fp8_oracle as fo
 from spikeinfer_b200.kernels import fp8 as k8
 from spikeinfer_b200.kernels import routing as kr
 
-from test_gpu_fp8_ops import BF, F32, FP8, check_route, gen
+from test_gpu_fp8_ops import BF, F32, FP8, check_linear, check_route, gen, operands
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,16 @@ def test_choices_among_few_and_saturated_logits(dev, experts, top, score):
     for bias in (None, torch.full((experts,), 2.0)):
         more = dict(score=score, bias=None if bias is None else bias.to(dev))
         check_route(kr.route_by_scores(logits.to(dev), top, **more), logits, top, **more)
+
+
+# ---- products ----------------------------------------------------------------------------------------------------------
+def test_a_product_of_many_tiles_by_pairs(dev):
+    """Some ten milliseconds in one launch, beyond any one wait's share: the last rows and features are right, nothing ran out, and again."""
+    n, k, f = 33_000, 18_944, 16_400
+    x, sx, w, sw = operands(n, k, f, dev, 7)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = k8.linear_fp8(x, sx, w, sw, status=status)
+    assert torch.equal(out, k8.linear_fp8(x, sx, w, sw, status=status)) and int(status.item()) == 0
+    fb = 16_256  # a block's first feature
+    for at in (slice(0, 20), slice(n - 140, n)):
+        check_linear(out[at, fb:], x[at], sx[:, at], w[fb:], sw[fb // 128:])
