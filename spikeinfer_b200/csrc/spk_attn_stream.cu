@@ -734,6 +734,7 @@ attn_tc_kernel(const AttnParams p, const StreamParams sp) {
         if (threadIdx.x < kWarps * kTcStages)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bars + threadIdx.x)));
         if (warp == 0) {
+            __syncwarp();
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(misc)), "r"(32 * kWarps));
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         }
@@ -936,7 +937,10 @@ attn_tc_kernel(const AttnParams p, const StreamParams sp) {
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(32 * kWarps));
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(32 * kWarps));
+    }
     if (!has_unit || unit >= n_units) return;
 
     // lane -> (head, quarter of the channels); digits d0..d3 of a sum recombine as d0 + 2^8 d1 + 2^16 d2 + 2^24 d3

@@ -39,8 +39,6 @@ struct Bars {
     uint32_t tmem;
 };
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // What CTA `rank` of the cluster has where this CTA has `addr`.
 __device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
     float v;
@@ -203,7 +201,6 @@ experts_kernel(const spk_experts_args a, const int blocks, const int ktiles) {
         }
     }
     if (S > 1) {
-        __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (warp >= 2) {  // every CTA adds and writes its own tokens
@@ -227,7 +224,6 @@ experts_kernel(const spk_experts_args a, const int blocks, const int ktiles) {
                 else store_plain<J>(a, row0 + j0, n, f, x, y);
             }
         }
-        __syncwarp();
         cluster_arrive();
         cluster_wait();  // no CTA leaves while its sums are being read
     }

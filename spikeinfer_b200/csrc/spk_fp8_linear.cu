@@ -79,8 +79,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // What CTA `rank` of the cluster has where this CTA has `addr`.
 __device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
     float v;
@@ -243,7 +241,6 @@ fp8_rows_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap
         }
     }
     if (S > 1) {
-        __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (warp >= 4) {  // every CTA adds and writes its own tokens
@@ -264,7 +261,6 @@ fp8_rows_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap
                 if (t0 + j0 + j < a.n && f < a.features) put(a, t0 + j0 + j, f, y);
             }
         }
-        __syncwarp();
         cluster_arrive();
         cluster_wait();  // no CTA leaves while its sums are being read
     }
@@ -432,6 +428,7 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
         if (CG == 1) {
             tmem_alloc(smem_u32(&bars->tmem), 512);
         } else {
+            __syncwarp();
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)), "r"(512) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
         }
@@ -574,7 +571,6 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
         }
     }
     if (S > 1) {
-        __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (warp >= 4) {  // every CTA adds and writes its own columns, two warps those of a token
@@ -603,8 +599,12 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
     tc_fence_after();
     if (threadIdx.x == 0 && *abort != 0) spk_flag(a.status, SPK_STATUS_DEVICE_WAIT_EXPIRED);
     if (warp == 0) {
-        if (CG == 1) tmem_dealloc(tmem, 512);
-        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        if (CG == 1) {
+            tmem_dealloc(tmem, 512);
+        } else {
+            __syncwarp();
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        }
     }
 }
 

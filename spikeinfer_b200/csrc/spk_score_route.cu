@@ -438,7 +438,8 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
             for (int k = 0; k <= behind; ++k) words[static_cast<int64_t>(e) * row + blockIdx.x + k] = k == 0 ? word[e] : 0u;
         return;
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
     int32_t *at = chosen + kTokens * a.top, *before = at + E;
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int all = 0, ahead = 0;
@@ -453,14 +454,14 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
     }
     __syncthreads();
     lay_out(a, blockIdx.x == 0, at, before, before + E);
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' words have been read
+    cluster_arrive();  // the others' words have been read
     const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens;
     const int pairs = static_cast<int>(min(a.n - first, static_cast<int64_t>(tokens))) * a.top;
     for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
         const int e = chosen[i];
         a.slots[first * a.top + i] = e >= 0 ? before[e] + __popc(word[e] & ((1u << (i / a.top)) - 1u)) : -1;
     }
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its words are being read
+    cluster_wait();  // no CTA leaves while its words are being read
 }
 
 __global__ void __launch_bounds__(kLayoutThreads)
