@@ -9,7 +9,8 @@
 //
 // A CTA's 32 tokens leave one word per expert, a bit for every token that chose it (a token chooses an expert once).  A pair's row is what the words ahead count, and the
 // bits below its own: no order of arrival enters, so the rows are the same every time.  Up to 128 tokens: a cluster's CTAs read one another's words, one launch.
-// More: score_layout_kernel, from the words in memory.
+// More: score_layout_kernel, from the words in memory; beyond kAllWords, where every CTA's counting of all of them would grow with the square of the tokens, from counts
+// by chunks of words that two more launches sum up (score_count_kernel, score_scan_kernel).
 #include "spk_experts.cuh"
 #include "spk_tensor.cuh"
 
@@ -22,6 +23,9 @@ constexpr int kMostCluster = 8;    // CTAs that hand out the rows among themselv
 constexpr int kMostWhole = 128;    // tokens of such a launch
 constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutWords = 8;    // words per CTA of the layout
+// Words that every CTA of the layout counts by itself; beyond, those of a chunk of kChunkWords (a multiple of kLayoutWords) are counted together.  us in all, by itself / by chunks: 32768 tokens
+// of 64 experts 34 / 37, of 256 87 / 78; 65536 68 / 62 and 190 / 147; 262144 381 / 239 and 1167 / 539.
+constexpr int kAllWords = 1024, kChunkWords = 64;
 
 // What makes a difference of two 32-bit scores settled: off times the larger (and the bias beside it) and kLeast.  The exponential's argument is off by |x| 2^-23 at most (a product, or a
 // difference and a product), which moves a sigmoid s by s (1 - s) |x| 2^-23 < 2^-25 and a softmax weight by d e^-d 2^-23 < 2^-24 (d: distance from the largest logit): kLeast.  The approximate
@@ -464,10 +468,58 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
     cluster_wait();  // no CTA leaves while its words are being read
 }
 
+// counts [chunk][expert] <- the pairs of a chunk's words, 16 lanes an expert.
 __global__ void __launch_bounds__(kLayoutThreads)
-score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ words, const int n_words, const int tokens) {
+score_count_kernel(const uint32_t* __restrict__ words, const int n_words, const int E, int32_t* __restrict__ counts) {
+    constexpr int L = kChunkWords / 4;
+    const int row = (n_words + 3) & ~3, q = blockIdx.x * L + threadIdx.x % L;
+    spk_grid_wait();
+    for (int e0 = 0; e0 < E; e0 += kLayoutThreads / L) {
+        const int e = e0 + threadIdx.x / L;
+        int c = 0;
+        if (e < E && q < row / 4) {
+            const uint4 u = __ldcg(reinterpret_cast<const uint4*>(words + static_cast<int64_t>(e) * row) + q);
+            c = __popc(u.x) + __popc(u.y) + __popc(u.z) + __popc(u.w);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int o = L / 2; o >= 1; o >>= 1) c += __shfl_xor_sync(~0u, c, o);
+        if (e < E && threadIdx.x % L == 0) counts[static_cast<int64_t>(blockIdx.x) * E + e] = c;
+    }
+}
+
+// counts [chunk][expert] <- the pairs ahead of a chunk, and behind the last chunk all pairs.  A lane per expert, a run of chunks per warp.
+__global__ void __launch_bounds__(1024)
+score_scan_kernel(int32_t* __restrict__ counts, const int chunks, const int E) {
+    __shared__ int32_t runs[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int lo = static_cast<int>(static_cast<int64_t>(chunks) * warp / 32), hi = static_cast<int>(static_cast<int64_t>(chunks) * (warp + 1) / 32);
+    int32_t* mine = counts + (e < E ? e : 0);
+    spk_grid_wait();
+    int sum = 0;
+#pragma unroll 8
+    for (int k = lo; k < hi; ++k) sum += e < E ? __ldcg(mine + static_cast<int64_t>(k) * E) : 0;
+    runs[warp][lane] = sum;
+    __syncthreads();
+    int ahead = 0;
+    for (int w = 0; w < warp; ++w) ahead += runs[w][lane];
+#pragma unroll 8
+    for (int k = lo; k < hi; ++k) {
+        if (e >= E) break;
+        const int c = __ldcg(mine + static_cast<int64_t>(k) * E);
+        mine[static_cast<int64_t>(k) * E] = ahead;
+        ahead += c;
+    }
+    if (warp == 31 && e < E) mine[static_cast<int64_t>(chunks) * E] = ahead;
+}
+
+// ALL: this CTA counts all words; else counts is score_scan_kernel's.
+template <bool ALL>
+__global__ void __launch_bounds__(kLayoutThreads)
+score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ words, const int n_words, const int tokens, const int32_t* __restrict__ counts, const int chunks) {
     extern __shared__ int32_t sm32[];  // [experts] twice, 32
     const int E = a.experts, w0 = blockIdx.x * kLayoutWords, row = (n_words + 3) & ~3, quads = row / 4;
+    const int chunk = w0 / kChunkWords, from = ALL ? 0 : chunk * (kChunkWords / 4), upto = ALL ? quads : w0 / 4;  // what is counted here
     int32_t *at = sm32, *before = at + E;
     spk_grid_wait();
     auto load = [&](int e, int q) { return __ldcg(reinterpret_cast<const uint4*>(words + static_cast<int64_t>(e) * row) + q); };
@@ -476,12 +528,12 @@ score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ 
     };
     // Lanes side by side take a row's words, 16 bytes each and about eight loads a lane: 8192 tokens' words of 256 experts in two passes.
     int side = 1;
-    while (side < 32 && 8 * side < quads) side <<= 1;
+    while (side < 32 && 8 * side < upto - from) side <<= 1;
     for (int e0 = 0; e0 < E; e0 += kLayoutThreads / side) {
         const int e = e0 + threadIdx.x / side;
         int all = 0, ahead = 0;
 #pragma unroll 8
-        for (int q = threadIdx.x % side; q < quads; q += side) {
+        for (int q = from + threadIdx.x % side; q < upto; q += side) {
             const int c = e < E ? count(load(e, q), 4) : 0;
             all += c;
             if (4 * q < w0) ahead += c;  // w0 is a multiple of four
@@ -492,8 +544,8 @@ score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ 
             ahead += __shfl_xor_sync(~0u, ahead, o);
         }
         if (e < E && threadIdx.x % side == 0) {
-            at[e] = all;
-            before[e] = ahead;
+            at[e] = ALL ? all : __ldcg(counts + static_cast<int64_t>(chunks) * E + e);
+            before[e] = ALL ? ahead : ahead + __ldcg(counts + static_cast<int64_t>(chunk) * E + e);
         }
     }
     __syncthreads();
@@ -517,6 +569,8 @@ score_layout_kernel(const spk_route_scores_args a, const uint32_t* __restrict__ 
 // them are on the chip at once (257 and 1024 rows 12.9 and 14.5 us, with 32 each 19.9 and 22.5).
 int tokens_of(int64_t n) { return n <= kMostWhole ? static_cast<int>((n + kMostCluster - 1) / kMostCluster) : n <= 148 * 8 ? 8 : n <= 148 * 16 ? 16 : kTokens; }
 int64_t words_of(int64_t n) { return n < 1 ? 0 : (n + tokens_of(n) - 1) / tokens_of(n); }
+int64_t word_bytes(int64_t n, int64_t experts) { return (words_of(n) + 3) / 4 * 16 * experts; }
+int64_t chunks_of(int64_t n) { return words_of(n) <= kAllWords ? 0 : (words_of(n) + kChunkWords - 1) / kChunkWords; }
 
 template <typename T, int P, bool WHOLE>
 int launch_select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStream_t s) {
@@ -559,7 +613,7 @@ int select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStr
 
 extern "C" int64_t spk_route_scores_workspace_bytes(int64_t n, int experts) {
     if (n <= kMostWhole || experts < 1) return 0;
-    return (words_of(n) + 3) / 4 * 16 * experts;
+    return word_bytes(n, experts) + (chunks_of(n) > 0 ? (chunks_of(n) + 1) * 4 * experts : 0);
 }
 
 extern "C" int spk_route_scores(const spk_route_scores_args* args, void* stream) {
@@ -585,6 +639,13 @@ extern "C" int spk_route_scores(const spk_route_scores_args* args, void* stream)
         const int rc = a.dtype == SPK_F32 ? select<float, false>(a, words, n_words, s) : select<__nv_bfloat16, false>(a, words, n_words, s);
         if (rc != SPK_OK) return rc;
     }
-    const int grid = n_words == 0 ? 1 : (n_words + kLayoutWords - 1) / kLayoutWords;
-    return spk_launch(score_layout_kernel, dim3(grid), kLayoutThreads, sizeof(int32_t) * (2 * a.experts + 32), s, n_words > 0, a, words, n_words, tokens_of(a.n));
+    const int grid = n_words == 0 ? 1 : (n_words + kLayoutWords - 1) / kLayoutWords, chunks = static_cast<int>(chunks_of(a.n));
+    const size_t bytes = sizeof(int32_t) * (2 * a.experts + 32);
+    int32_t* counts = nullptr;
+    if (chunks == 0) return spk_launch(score_layout_kernel<true>, dim3(grid), kLayoutThreads, bytes, s, n_words > 0, a, words, n_words, tokens_of(a.n), counts, chunks);
+    counts = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a.workspace) + word_bytes(a.n, a.experts));
+    int rc = spk_launch(score_count_kernel, dim3(chunks), kLayoutThreads, 0, s, true, words, n_words, a.experts, counts);
+    if (rc == SPK_OK) rc = spk_launch(score_scan_kernel, dim3((a.experts + 31) / 32), 1024, 0, s, true, counts, chunks, a.experts);
+    if (rc == SPK_OK) rc = spk_launch(score_layout_kernel<false>, dim3(grid), kLayoutThreads, bytes, s, true, a, words, n_words, tokens_of(a.n), counts, chunks);
+    return rc;
 }

@@ -118,3 +118,68 @@ def test_a_product_of_many_tiles_by_pairs(dev):
     fb = 16_256  # a block's first feature
     for at in (slice(0, 20), slice(n - 140, n)):
         check_linear(out[at, fb:], x[at], sx[:, at], w[fb:], sw[fb // 128:])
+
+
+# ---- rows of many tokens' choices -------------------------------------------------------------------------------------
+def rows_in_order(r, experts):
+    """slots and segs follow from the ids: segments of multiples of eight rows, the pairs of an expert in their order."""
+    ids = r.ids.cpu().long()
+    n, top = ids.shape
+    flat = torch.where(ids < 0, experts, ids).flatten()
+    counts = torch.bincount(flat, minlength=experts + 1)[:experts]
+    first = torch.cumsum((counts + 7) // 8 * 8, 0) - (counts + 7) // 8 * 8
+    order = torch.sort(flat, stable=True).indices
+    place = torch.empty_like(flat)
+    place[order] = torch.arange(n * top)
+    e = flat.clamp(max=experts - 1)
+    slots = torch.where(flat < experts, first[e] + place - (torch.cumsum(counts, 0) - counts)[e], -1)
+    assert torch.equal(r.slots.cpu().long().flatten(), slots) and torch.equal(r.segs.cpu().long(), torch.stack((first, counts), 1))
+
+
+@pytest.mark.parametrize("n,experts,top", [(2369, 24, 3), (5000, 40, 4), (5000, 256, 8)])
+def test_routes_of_32_tokens_a_word(dev, n, experts, top):
+    logits = torch.randn(n, experts, generator=gen(n))
+    groups, top_groups = (8, 4) if experts == 256 else (1, 1)
+    more = dict(score="sigmoid", groups=groups, top_groups=top_groups)
+    r = kr.route_by_scores(logits.to(dev), top, **more)
+    check_route(r, logits, top, **more)
+    rows_in_order(r, experts)
+
+
+@pytest.mark.parametrize("n,experts,top", [(32_768, 16, 2), (32_769, 16, 2), (70_001, 64, 6), (300_000, 33, 1), (1_000_003, 8, 2)])
+def test_routes_beyond_what_a_cta_counts(dev, n, experts, top):
+    """More words than every CTA of the layout counts by itself (1024): counts by chunks, the last of each cut short."""
+    g = torch.Generator(device=dev).manual_seed(n)
+    logits = torch.randn(n, experts, generator=g, device=dev)
+    active = (torch.rand(n, generator=g, device=dev) < 0.97).to(torch.int32)
+    logits[torch.rand(n, generator=g, device=dev) < 0.01] = -float("inf")
+    r = kr.route_by_scores(logits, top, active=active)
+    rows_in_order(r, experts)
+    want = torch.sort(logits.double().softmax(1), dim=1, descending=True, stable=True).indices[:, :top]
+    there = (active == 1) & (logits[:, 0] > -float("inf"))
+    assert torch.equal(r.ids[there].long(), want[there]) and (r.ids[~there] == -1).all()
+    again = kr.route_by_scores(logits, top, active=active)
+    assert torch.equal(r.slots, again.slots) and torch.equal(r.segs, again.segs)
+
+
+def test_routes_of_many_tokens_in_a_graph_beside_others(dev):
+    n, experts = 50_000, 48
+    x, other = (torch.randn(n, experts, generator=torch.Generator(device=dev).manual_seed(s), device=dev) for s in (1, 2))
+    want = [kr.route_by_scores(t, 4) for t in (x, other)]
+    held = x.clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        kr.route_by_scores(held, 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = kr.route_by_scores(held, 4)
+    for t, w in ((other, want[1]), (x, want[0])):
+        held.copy_(t)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        beside = [kr.route_by_scores(other, 4) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(captured.slots, w.slots) and torch.equal(captured.segs, w.segs) and torch.equal(captured.weights, w.weights)
+        assert all(torch.equal(b.slots, want[1].slots) and torch.equal(b.segs, want[1].segs) for b in beside)
