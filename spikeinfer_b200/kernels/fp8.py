@@ -43,13 +43,15 @@ def one_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
 
 @torch.no_grad()
 def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """A weight matrix ``[features, k]`` as e4m3 values and scales for blocks of 128 x 128, for :func:`linear_fp8`; done once, when a model is loaded."""
+    """A weight matrix ``[features, k]`` as e4m3 values and scales for blocks of 128 x 128, for :func:`linear_fp8`; done once, when a model is loaded.  As in the
+    activations, NaN stays NaN and is not the largest of its block, and an infinity counts as the largest finite value."""
     f, k = w.shape
     fb, kb = -(-f // BLOCK), -(-k // BLOCK)
     x = w.new_zeros((fb * BLOCK, kb * BLOCK), dtype=torch.float32)
     x[:f, :k] = w
     x = x.view(fb, BLOCK, kb, BLOCK)
-    scales = x.abs().amax(dim=(1, 3)).clamp(min=2.0 ** -100) / 448.0
+    most = x.abs().nan_to_num_(nan=0.0, posinf=torch.finfo(torch.float32).max).amax(dim=(1, 3))
+    scales = most.clamp(min=2.0 ** -100) / 448.0
     out = rows_fp8(f, k, w.device)
     out.copy_((x / scales[:, None, :, None]).clamp(-448.0, 448.0).view(fb * BLOCK, kb * BLOCK)[:f, :k])
     return out, scales.contiguous()

@@ -1,7 +1,9 @@
 """CPU: host sides of the 8-bit operators and of the routes by scores: workspaces, weights, forms."""
 from __future__ import annotations
 
+import torch
 
+from spikeinfer_b200.kernels import fp8 as k8
 
 
 def test_workspace_of_many_tokens_holds_counts_by_chunks(lib):
@@ -14,3 +16,25 @@ def test_workspace_of_many_tokens_holds_counts_by_chunks(lib):
         for n in (32_769, 70_000, 1 << 24):
             words = -(-n // 32)
             assert need(n, experts) == -(-words // 4) * 16 * experts + (-(-words // 64) + 1) * 4 * experts
+
+
+def test_weights_that_are_not_finite_stay_alone():
+    """NaN is NaN and not the largest of its block, an infinity counts as the largest finite value: the rule of the activations."""
+    inf, nan, top = float("inf"), float("nan"), torch.finfo(torch.float32).max
+    for dtype in (torch.float32, torch.bfloat16):
+        w = torch.randn(200, 300, generator=torch.Generator().manual_seed(1)).to(dtype)
+        w[3, 5] = 0.0
+        want, _ = k8.quantize_weight(w)
+        bad = w.clone()
+        bad[3, 5], bad[150, 20], bad[130, 299] = nan, inf, -inf
+        bad[:128, 256:] = nan
+        q, s = k8.quantize_weight(bad)
+        values = q.float()
+        assert torch.isfinite(s).all() and float(s[0, 2]) == float(torch.tensor(2.0 ** -100) / 448)
+        assert values[3, 5].isnan() and values[:128, 256:].isnan().all() and int(values.isnan().sum()) == 1 + 128 * 44
+        assert float(s[1, 0]) == float(s[1, 2]) == float(torch.tensor(top) / 448) and values[150, 20] == 448 and values[130, 299] == -448
+        rest = torch.ones(200, 300, dtype=torch.bool)  # blocks without an infinity: as they were
+        rest[3, 5] = False
+        rest[:128, 256:] = rest[128:, :128] = rest[128:, 256:] = False
+        assert torch.equal(values[rest], want.float()[rest])
+        assert (values[128:, :128] == 0).sum() >= 72 * 128 - 1  # next to 3e38 there is nothing left of the others
