@@ -27,11 +27,13 @@ def _scales(n: int, width: int, device) -> torch.Tensor:
     return torch.empty_strided((-(-width // BLOCK), n), (n, 1), dtype=_F32, device=device)
 
 
-def _is_rows(t: torch.Tensor, what: str) -> None:
+def _row_stride(t: torch.Tensor, what: str) -> int:
     if t.ndim == 2 and t.dtype is FP8:
-        (row, column), width = t.stride(), t.shape[1]
+        (row, column), (n, width) = t.stride(), t.shape
+        if n <= 1 or width == 1:  # torch gives an axis of one any stride
+            row, column = row if n > 1 else -(-width // 16) * 16, 1 if width == 1 else column
         if column == 1 and row >= width > 0 and not row % 16 and not t.data_ptr() % 16:
-            return
+            return row
     raise ValueError(f"{what} must be e4m3 [rows, columns] with unit column stride and rows that start on 16-byte boundaries")
 
 
@@ -108,12 +110,12 @@ def quantize_fp8(z: torch.Tensor, act: str = "none") -> tuple[torch.Tensor, torc
     _lib.require_cuda(z, "quantize_fp8 input")
     if act not in _ACTS:
         raise ValueError(f"unknown activation {act!r} (known: {', '.join(_ACTS)})")
-    if z.ndim != 2 or z.dtype not in _FLOATS or z.stride(1) != 1 or z.stride(0) < z.shape[1] or z.shape[1] < 1 \
+    if z.ndim != 2 or z.dtype not in _FLOATS or z.shape[1] < 1 or (z.shape[1] > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < z.shape[1]) \
             or (act == "silu_gate" and z.shape[1] % 2):
         raise ValueError("z must be [n, width], fp32 or bf16, with unit column stride; an even width for the gate")
     n, width = z.shape[0], z.shape[1] // (2 if act == "silu_gate" else 1)
     q, scales = rows_fp8(n, width, z.device), _scales(n, width, z.device)
-    a = _lib.QuantizeFp8Args(z=z.data_ptr(), q=q.data_ptr(), scales=scales.data_ptr(), z_stride=z.stride(0), q_stride=q.stride(0), scale_stride=n, n=n,
+    a = _lib.QuantizeFp8Args(z=z.data_ptr(), q=q.data_ptr(), scales=scales.data_ptr(), z_stride=max(z.shape[1], z.stride(0)), q_stride=q.stride(0), scale_stride=n, n=n,
                              width=width, act=_ACTS[act], dtype=_lib.dtype_code(z.dtype))
     _call("spk_quantize_fp8", a, z.device)
     return q, scales
@@ -124,8 +126,7 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     """``x w^T`` of e4m3 rows ``[n, k]`` and weights ``[features, k]`` with their scales, 32-bit sums, in ``out_dtype`` (fp32 or bf16).  ``out`` may be a column
     range of a row-major matrix."""
     _lib.require_cuda(x, "linear_fp8 input")
-    _is_rows(x, "x")
-    _is_rows(w, "w")
+    x_stride, w_stride = _row_stride(x, "x"), _row_stride(w, "w")
     (n, k), features = x.shape, w.shape[0]
     blocks = -(-k // BLOCK)
     if w.shape[1] != k or features < 1:
@@ -141,7 +142,7 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("out must be [n, features] in out_dtype, fp32 or bf16, with unit column stride")
     one_device(x.device, x_scales, w, w_scales, out, status)
     a = _lib.LinearFp8Args(x=x.data_ptr(), w=w.data_ptr(), x_scales=x_scales.data_ptr(), w_scales=w_scales.data_ptr(), out=out.data_ptr(),
-                           x_stride=x.stride(0), w_stride=w.stride(0), x_scale_stride=max(n, x_scales.stride(0)), w_scale_stride=blocks,
+                           x_stride=x_stride, w_stride=w_stride, x_scale_stride=max(n, x_scales.stride(0)), w_scale_stride=blocks,
                            out_stride=max(features, out.stride(0)), n=n, k=k, features=features, out_dtype=_lib.dtype_code(out_dtype),
                            status=_ptr(status))
     _call("spk_linear_fp8", a, x.device)

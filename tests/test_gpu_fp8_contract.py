@@ -183,3 +183,24 @@ def test_routes_of_many_tokens_in_a_graph_beside_others(dev):
         torch.cuda.synchronize()
         assert torch.equal(captured.slots, w.slots) and torch.equal(captured.segs, w.segs) and torch.equal(captured.weights, w.weights)
         assert all(torch.equal(b.slots, want[1].slots) and torch.equal(b.segs, want[1].segs) for b in beside)
+
+
+# ---- single rows -----------------------------------------------------------------------------------------------------
+def test_the_stride_of_a_single_row_is_of_no_account(dev):
+    one = lambda t, stride: t.as_strided((1, t.shape[1]), (stride, 1))
+    for act in ("none", "silu_gate"):
+        z = torch.randn(1, 300, generator=gen(2)).to(dev)
+        want, scales = k8.quantize_fp8(z, act)
+        got, s = k8.quantize_fp8(one(z, 1), act)
+        assert torch.equal(got.float(), want.float()) and torch.equal(s, scales)
+    column = torch.randn(5, 7, generator=gen(3)).to(dev)[:, 2:3]  # nor that of a single column
+    got, s = k8.quantize_fp8(column)
+    want, scales = k8.quantize_fp8(column.clone())
+    assert torch.equal(got.float(), want.float()) and torch.equal(s, scales)
+    x, sx, w, sw = operands(1, 200, 1, dev, 4)
+    want = k8.linear_fp8(x, sx, w, sw)
+    for stride in (1, 200, 208):
+        assert torch.equal(k8.linear_fp8(one(x, stride), sx, one(w, stride), sw), want)
+    for bad in (one(x, 200)[:, 8:], torch.empty(2, 200, dtype=FP8, device=dev)[:, :40].t(), torch.empty(2, 200, dtype=FP8, device=dev)[:, :45]):
+        with pytest.raises(ValueError):
+            k8.linear_fp8(bad, sx, w, sw)
