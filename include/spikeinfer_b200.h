@@ -762,7 +762,8 @@ int spk_quantize_fp8(const spk_quantize_fp8_args* args, void* stream);
 
 /* out[t, f] = sum_b x_scales[b * x_scale_stride + t] * w_scales[(f / 128) * w_scale_stride + b] * (sum of x[t, c] w[f, c] over columns c of block b), sums
  * in 32 bits, out in out_dtype (SPK_F32 or SPK_BF16) with row stride out_stride elements.  x [n, k] and w [features, k] in e4m3, 16-byte aligned, row
- * strides x_stride and w_stride bytes.  The result does not depend on timing. */
+ * strides x_stride and w_stride bytes.  The product of two scales need not be a 32-bit number (one below 2^-126 counts to within 2^-150).  The result does not depend on
+ * timing. */
 typedef struct spk_linear_fp8_args {
     const void* x;
     const void* w;

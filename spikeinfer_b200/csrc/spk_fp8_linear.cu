@@ -14,6 +14,8 @@
 // Measured on the way, us for 8192 x 3584 x 18944: one accumulating warpgroup per feature block 1680; products of pairs (fma.rn.f32x2) 656, one by one 606; barriers for every
 // block's scales 703, for eight blocks 600; an arrival with cluster scope on the pair's barrier 1240, without 640; 16 writing warps 606, eight 600.
 #include <cuda.h>
+#include <cuda_fp8.h>
+#include <float.h>
 
 #include "spk_dense.cuh"
 #include "spk_tensor.cuh"
@@ -46,6 +48,7 @@ struct Bars {
     uint64_t full[10], free[10], sums[4], drained[4], factors[8], used[8], done;
     int abort;
     uint32_t tmem;
+    int odd;  // rows: a token may be far
 };
 
 // kind::f8f6f4 instruction descriptor: e4m3 operands, contiguous along k, fp32 accumulator.
@@ -91,9 +94,48 @@ __device__ __forceinline__ void put(const spk_linear_fp8_args& a, int64_t t, int
     else static_cast<__nv_bfloat16*>(a.out)[t * a.out_stride + f] = __float2bfloat16_rn(v);
 }
 
+// A block's sum is multiplied by the product of its scales.  Where that is beyond the 32-bit numbers while both scales are not (1e20 times 1e20, beside a sum of zero too), what a thread has
+// added up is put aside, and its outputs are summed up here from the operands, some hundred times as slow: a sum times the smaller scale, times the larger one, so that nothing on the way
+// overflows unless the term does.  (A branch for every block in the loops that read tensor memory took 2 to 12 % of all products.)  A product below the normal numbers is taken as it is, to
+// within 2^-150: scales of 2^-100 / 448, those of blocks of zeros, are met beside small ones.
+__device__ __forceinline__ bool is_far(float x, float w) { return fabsf(x * w) == INFINITY && fabsf(x) <= FLT_MAX && fabsf(w) <= FLT_MAX; }
+__device__ __forceinline__ bool may_be_far(float product) { return !(fabsf(product) <= FLT_MAX); }  // or one of the scales is not finite
+__device__ __noinline__ bool has_far(const spk_linear_fp8_args& a, int64_t t, int64_t f, int kb, int kn) {
+    if (t >= a.n || f >= a.features) return false;
+    bool far = false;
+    for (int b = kb; b < kb + kn && !far; ++b) far = is_far(a.x_scales[b * a.x_scale_stride + t], a.w_scales[f / kBlock * a.w_scale_stride + b]);
+    return far;
+}
+__device__ __noinline__ float far_sum(const spk_linear_fp8_args& a, int64_t t, int64_t f, int kb, int kn) {
+    if (t >= a.n || f >= a.features) return 0.0f;
+    const uint8_t *x = static_cast<const uint8_t*>(a.x) + t * a.x_stride, *w = static_cast<const uint8_t*>(a.w) + f * a.w_stride;
+    auto two = [](uint32_t v) { return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3))); };
+    float y = 0.0f;
+    for (int b = kb; b < kb + kn; ++b) {
+        const int64_t c0 = static_cast<int64_t>(b) * kBlock, c1 = min(c0 + kBlock, a.k);
+        float s = 0.0f;
+        int64_t c = c0;
+        for (; c + 16 <= c1; c += 16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(x + c), v = *reinterpret_cast<const uint4*>(w + c);
+            const uint32_t p[4] = {u.x, u.y, u.z, u.w}, q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 e = two(p[i / 2] >> (i % 2 * 16) & 0xffffu), g = two(q[i / 2] >> (i % 2 * 16) & 0xffffu);
+                s = fmaf(e.x, g.x, s);
+                s = fmaf(e.y, g.y, s);
+            }
+        }
+        for (; c < c1; ++c) s = fmaf(two(x[c]).x, two(w[c]).x, s);
+        const float sx = a.x_scales[b * a.x_scale_stride + t], sw = a.w_scales[f / kBlock * a.w_scale_stride + b], m = sx * sw;
+        const bool x_first = fabsf(sx) < fabsf(sw);
+        y = is_far(sx, sw) ? fmaf(s * (x_first ? sx : sw), x_first ? sw : sx, y) : fmaf(s, m, y);
+    }
+    return y;
+}
+
 template <int TN, int S>
 __global__ void __launch_bounds__(Shape<TN>::kThreads, 1)
-fp8_rows_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const int blocks) {
+fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const int blocks) {
     using Sh = Shape<TN>;
     constexpr int NS = Sh::NS, NB = Sh::NB;
     static_assert(S == 1 || TN * 128 * 4 <= NS * Sh::kStage, "partial sums take the stages' place");
@@ -121,7 +163,7 @@ fp8_rows_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap
             mbar_init(smem_u32(&bars->used[i]), Sh::kWriters);
         }
         mbar_init(smem_u32(&bars->done), 1);
-        bars->abort = 0;
+        bars->abort = bars->odd = 0;
     }
     if (warp == 0) tmem_alloc(smem_u32(&bars->tmem), Sh::kColumns);
     fence_async_shared();
@@ -182,8 +224,11 @@ fp8_rows_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap
 #pragma unroll
             for (int i = 0; i < kRun; ++i)
 #pragma unroll
-                for (int j = 0; j < R; ++j)
-                    if (32 * j + lane < TN) ring[(at * kRun + i) * TN + 32 * j + lane] = u[i][j] * v[i];
+                for (int j = 0; j < R; ++j) {
+                    const float m = u[i][j] * v[i];
+                    if (may_be_far(m)) bars->odd = 1;
+                    if (32 * j + lane < TN) ring[(at * kRun + i) * TN + 32 * j + lane] = m;
+                }
             mbar_arrive(smem_u32(&bars->factors[at]));
         }
     } else {  // a feature per lane, 32 tokens (or all 16) per warp
@@ -234,10 +279,16 @@ fp8_rows_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap
 #pragma unroll
             for (int j = 0; j < C; ++j)
                 if (ok && t0 + j0 + j < a.n && f < a.features) put(a, t0 + j0 + j, f, acc[j]);
+            if (ok && bars->odd != 0)
+                for (int j = 0; j < C; ++j)
+                    if (has_far(a, t0 + j0 + j, f, kb, kn)) put(a, t0 + j0 + j, f, far_sum(a, t0 + j0 + j, f, kb, kn));
         } else {  // [token][128 features]
             float* sums = reinterpret_cast<float*>(base) + j0 * 128 + quad * 32 + lane;
 #pragma unroll
             for (int j = 0; j < C; ++j) sums[j * 128] = ok ? acc[j] : 0.0f;
+            if (ok && bars->odd != 0)
+                for (int j = 0; j < C; ++j)
+                    if (has_far(a, t0 + j0 + j, f, kb, kn)) sums[j * 128] = far_sum(a, t0 + j0 + j, f, kb, kn);
         }
     }
     if (S > 1) {
@@ -391,7 +442,7 @@ __device__ __forceinline__ void put_row(const spk_linear_fp8_args& a, int vec, i
 
 template <int NF, int CG, int S>
 __global__ void __launch_bounds__(kTileThreads, 1)
-fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const int blocks, const int m_tiles,
+fp8_tiles_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const int blocks, const int m_tiles,
                  const int n_tiles, const int vec, const int vec_scales) {
     using Sh = Tile<NF, CG>;
     constexpr int NS = Sh::NS, NB = Sh::NB, H = 4 * NF / kWriters;  // columns of a thread
@@ -520,7 +571,7 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const uint32_t drained = CG == 2 ? at_rank(smem_u32(&bars->drained[0]), 0) : smem_u32(&bars->drained[0]);
         int c = 0, g = 0;
-        bool ok = true;
+        bool ok = true, odd = false;
         for (int tile = first; tile < tiles && ok; tile += stride) {
             float acc[H];
 #pragma unroll
@@ -530,6 +581,7 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
                 if (k % kGroup == 0) ok = mbar_wait(smem_u32(&bars->factors[g % kGroups]), (g / kGroups) & 1, abort);
                 const float* scales = ring + (g % kGroups * kGroup + k % kGroup) * 132;
                 const float m = scales[r] * scales[128 + half * H / 128];
+                odd = odd || may_be_far(m);
                 ok = __all_sync(~0u, ok && mbar_wait(smem_u32(&bars->sums[b]), (c / NB) & 1, abort));
                 if (!ok) break;
                 tc_fence_after();
@@ -557,8 +609,8 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
                 }
                 if (last) ++g;
             }
+            const int64_t t = static_cast<int64_t>(m_of(tile)) * 128 * CG + rank * 128 + r, f = static_cast<int64_t>(n_of(tile)) * NF + half * H;
             if (S == 1) {
-                const int64_t t = static_cast<int64_t>(m_of(tile)) * 128 * CG + rank * 128 + r, f = static_cast<int64_t>(n_of(tile)) * NF + half * H;
                 if (ok && t < a.n) {
 #pragma unroll
                     for (int j = 0; j < H; j += 32) put_row<32>(a, vec, t, f + j, acc + j);
@@ -567,6 +619,15 @@ fp8_tiles_kernel(const spk_linear_fp8_args a, const __grid_constant__ CUtensorMa
                 float* sums = reinterpret_cast<float*>(base) + half * H * 128 + r;
 #pragma unroll
                 for (int j = 0; j < H; ++j) sums[j * 128] = ok ? acc[j] : 0.0f;
+                if (ok && odd && has_far(a, t, f, kb, kn))
+                    for (int j = 0; j < H; ++j) sums[j * 128] = far_sum(a, t, f + j, kb, kn);
+            }
+        }
+        if (S == 1 && ok && odd) {  // behind the last tile, where no other warp waits for this one
+            for (int tile = first; tile < tiles; tile += stride) {
+                const int64_t t = static_cast<int64_t>(m_of(tile)) * 128 * CG + rank * 128 + r, f = static_cast<int64_t>(n_of(tile)) * NF + half * H;
+                if (has_far(a, t, f, kb, kn))
+                    for (int j = 0; j < H && f + j < a.features; ++j) put(a, t, f + j, far_sum(a, t, f + j, kb, kn));
             }
         }
     }

@@ -204,3 +204,40 @@ def test_the_stride_of_a_single_row_is_of_no_account(dev):
     for bad in (one(x, 200)[:, 8:], torch.empty(2, 200, dtype=FP8, device=dev)[:, :40].t(), torch.empty(2, 200, dtype=FP8, device=dev)[:, :45]):
         with pytest.raises(ValueError):
             k8.linear_fp8(bad, sx, w, sw)
+
+
+# ---- scales far from one ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,k,f", [(5, 300, 200), (40, 2100, 300), (130, 400, 300), (130, 2100, 200), (600, 300, 2600), (1171, 200, 4864), (2600, 260, 4000)])
+def test_products_of_scales_beyond_32_bits(dev, n, k, f):
+    """A block's two scales need not have a product in 32 bits: what counts is the block's term."""
+    x, sx, w, sw = operands(n, k, f, dev, n)
+    sx.fill_(1.0)
+    sw.fill_(1.0)
+    top = 2.0 ** 70
+    sx[1], sw[:, 1] = top, top  # block 1: 2^140, beside nothing, and beside products of 2^-18
+    x[:, 128:256] = 0.0
+    x[1::2, 130] = 2.0 ** -9
+    w[:, 130] = 2.0 ** -9
+    out = k8.linear_fp8(x, sx, w, sw, out_dtype=F32)
+    assert torch.isfinite(out[1::2]).all() and (out[1::2] > 2.0 ** 121).all()
+    check_linear(out, x, sx, w, sw)
+    near = k8.linear_fp8(x, torch.ones_like(sx), w, sw, out_dtype=F32)
+    sx[1, 1:] = 1.0  # row 0 alone is far: the others keep their bits
+    assert torch.equal(k8.linear_fp8(x, sx, w, sw, out_dtype=F32)[1:], near[1:])
+    # far below: products of 2^-138, of which 32 bits hold a few, known to within 2^-150 each
+    g = torch.Generator(device=dev).manual_seed(k)
+    x, _, w, _ = operands(n, k, f, dev, n + 1)
+    size = x.double().cpu().abs() @ w.double().cpu().abs().t()
+    sx.copy_((0.5 + torch.rand(sx.shape, generator=g, device=dev)) * 2.0 ** -72)
+    sw.copy_((0.5 + torch.rand(sw.shape, generator=g, device=dev)) * 2.0 ** -66)
+    want, _ = fo.linear(x.cpu(), sx.cpu(), w.cpu(), sw.cpu())
+    off = (k8.linear_fp8(x, sx, w, sw, out_dtype=F32).double().cpu() - want).abs()
+    assert (off <= 2.0 ** -150 * size * (1 + 132 * 2.0 ** -23) + 2.0 ** -16 * 2.0 ** -136 * size).all()  # 132 x 2^-23 of the terms: under 2^-16 of them, scales under 1.5^2 x 2^-138
+    # blocks of zeros as quantize_fp8 leaves them, beside scales of any size; a scale of zero is zero beside any other
+    sx.fill_(1.0)
+    sw.fill_(1.0)
+    sx[1], x[:, 128:256] = 2.0 ** -100 / 448, 0.0
+    sw[:, 1] = 2.0 ** -40
+    check_linear(k8.linear_fp8(x, sx, w, sw, out_dtype=F32), x, sx, w, sw)
+    sx[0], sw[:, 0] = 0.0, 2.0 ** 120
+    check_linear(k8.linear_fp8(x, sx, w, sw, out_dtype=F32), x, sx, w, sw)
