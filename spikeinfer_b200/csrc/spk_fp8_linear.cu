@@ -146,7 +146,6 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = static_cast<int>(blockIdx.x) % S;
     const int fb = blockIdx.x / S;                                        // block of 128 features
-    const int64_t t0 = static_cast<int64_t>(blockIdx.y) * TN;
     const int kb = blocks * part / S, kn = blocks * (part + 1) / S - kb;  // this CTA's blocks of k, at least one
     const int groups = (kn + kRun - 1) / kRun;
     if (threadIdx.x == 0) {
@@ -181,7 +180,7 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
                 const uint32_t bar = smem_u32(&bars->full[s]), dst = smem_u32(base + s * Sh::kStage);
                 mbar_expect(bar, Sh::kStage);
                 tma_load(dst, &w_map, (kb + k) * kBlock, fb * 128, bar);
-                tma_load(dst + kTileW, &x_map, (kb + k) * kBlock, static_cast<int>(t0), bar);
+                tma_load(dst + kTileW, &x_map, (kb + k) * kBlock, 0, bar);
                 issued = k + 1;
             }
             if (*abort != 0)  // copies in flight land before the CTA's shared memory is given up
@@ -215,10 +214,10 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
 #pragma unroll
             for (int i = 0; i < kRun; ++i) {
                 const int k = g * kRun + i;
-                const float* x = a.x_scales + (kb + k) * a.x_scale_stride + t0;
+                const float* x = a.x_scales + (kb + k) * a.x_scale_stride;
                 v[i] = k < kn ? w[k] : 0.0f;
 #pragma unroll
-                for (int j = 0; j < R; ++j) u[i][j] = k < kn && 32 * j + lane < TN && t0 + 32 * j + lane < a.n ? x[32 * j + lane] : 0.0f;
+                for (int j = 0; j < R; ++j) u[i][j] = k < kn && 32 * j + lane < TN && 32 * j + lane < a.n ? x[32 * j + lane] : 0.0f;
             }
             if (g >= Sh::kRing && !__all_sync(~0u, mbar_wait(smem_u32(&bars->used[at]), ((g / Sh::kRing) - 1) & 1, abort))) break;
 #pragma unroll
@@ -278,17 +277,17 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
         if (S == 1) {
 #pragma unroll
             for (int j = 0; j < C; ++j)
-                if (ok && t0 + j0 + j < a.n && f < a.features) put(a, t0 + j0 + j, f, acc[j]);
+                if (ok && j0 + j < a.n && f < a.features) put(a, j0 + j, f, acc[j]);
             if (ok && bars->odd != 0)
                 for (int j = 0; j < C; ++j)
-                    if (has_far(a, t0 + j0 + j, f, kb, kn)) put(a, t0 + j0 + j, f, far_sum(a, t0 + j0 + j, f, kb, kn));
+                    if (has_far(a, j0 + j, f, kb, kn)) put(a, j0 + j, f, far_sum(a, j0 + j, f, kb, kn));
         } else {  // [token][128 features]
             float* sums = reinterpret_cast<float*>(base) + j0 * 128 + quad * 32 + lane;
 #pragma unroll
             for (int j = 0; j < C; ++j) sums[j * 128] = ok ? acc[j] : 0.0f;
             if (ok && bars->odd != 0)
                 for (int j = 0; j < C; ++j)
-                    if (has_far(a, t0 + j0 + j, f, kb, kn)) sums[j * 128] = far_sum(a, t0 + j0 + j, f, kb, kn);
+                    if (has_far(a, j0 + j, f, kb, kn)) sums[j * 128] = far_sum(a, j0 + j, f, kb, kn);
         }
     }
     if (S > 1) {
@@ -303,13 +302,13 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
 #pragma unroll
             for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int r = 0; r < S; ++r) v[j][r] = t0 + j0 + j < a.n ? cluster_load(own + j * 512, r) : 0.0f;
+                for (int r = 0; r < S; ++r) v[j][r] = j0 + j < a.n ? cluster_load(own + j * 512, r) : 0.0f;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 float y = v[j][0];
 #pragma unroll
                 for (int r = 1; r < S; ++r) y += v[j][r];
-                if (t0 + j0 + j < a.n && f < a.features) put(a, t0 + j0 + j, f, y);
+                if (j0 + j < a.n && f < a.features) put(a, j0 + j, f, y);
             }
         }
         cluster_arrive();
@@ -695,21 +694,21 @@ bool encode(CUtensorMap* map, const void* p, int64_t rows, int64_t columns, int6
 
 int aligned_scales(const spk_linear_fp8_args& a) { return reinterpret_cast<uintptr_t>(a.x_scales) % 16 == 0 && a.x_scale_stride % 4 == 0; }
 
-template <int TN, int S>
+template <int TN, int S>  // n <= TN
 int launch_rows(const spk_linear_fp8_args& a, cudaStream_t s) {
     constexpr int bytes = Shape<TN>::kBytes;
     static_assert(sizeof(Bars) <= 1024 && bytes <= 227 * 1024, "shared memory");
     CUtensorMap w_map, x_map;
     if (!encode(&w_map, a.w, a.features, a.k, a.w_stride, 128) || !encode(&x_map, a.x, a.n, a.k, a.x_stride, TN)) return SPK_ERR_UNSUPPORTED;
     const int blocks = static_cast<int>((a.k + kBlock - 1) / kBlock);
-    const int64_t fblocks = (a.features + 127) / 128, runs = (a.n + TN - 1) / TN;
-    if (fblocks * S > 0x7fffffff || runs > 65535) return SPK_ERR_TOO_LARGE;
+    const int64_t fblocks = (a.features + 127) / 128;
+    if (fblocks * S > 0x7fffffff) return SPK_ERR_TOO_LARGE;
     auto kernel = fp8_rows_kernel<TN, S>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return spk_set_cuda_error(e);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1] = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(fblocks * S), static_cast<unsigned>(runs));
+    cfg.gridDim = dim3(static_cast<unsigned>(fblocks * S));
     cfg.blockDim = dim3(Shape<TN>::kThreads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = s;
