@@ -21,6 +21,7 @@ using namespace spk_tc;
 constexpr int kTokens = 32;        // per CTA of the selection, at most: the bits of a word
 constexpr int kMostCluster = 8;    // CTAs that hand out the rows among themselves
 constexpr int kMostWhole = 128;    // tokens of such a launch
+constexpr int kWholeTokens = kMostWhole / kMostCluster;  // of a CTA of it
 constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutWords = 8;    // words per CTA of the layout
 // Words that every CTA of the layout counts by itself; beyond, those of a chunk of kChunkWords (a multiple of kLayoutWords) are counted together.  us in all, by itself / by chunks: 32768 tokens
@@ -368,15 +369,16 @@ __device__ __forceinline__ uint32_t cluster_load(const uint32_t* p, uint32_t ran
     return v;
 }
 
-// WHOLE: the grid is one cluster and hands out the rows as well.
+// WHOLE: the grid is one cluster and hands out the rows as well; at most kWholeTokens tokens, a warp each, so that a thread may have 128 registers and few spill (64 of them, a bound of
+// 1024 threads: 64 tokens of 256 experts 12.4 us against 11.7, of 384 16.5 against 14.9).
 template <typename T, int P, bool WHOLE>
-__global__ void __launch_bounds__(WHOLE ? 1024 : 512, WHOLE ? 1 : 2)
+__global__ void __launch_bounds__(512, WHOLE ? 1 : 2)
 score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* words, const int n_words, const int tokens) {
     extern __shared__ double sm[];
     const int E = a.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     double* c64 = sm + static_cast<int64_t>(warp) * 2 * E;  // also the 32-bit scores
     uint32_t* word = reinterpret_cast<uint32_t*>(sm + static_cast<int64_t>(warps) * 2 * E);
-    int32_t* chosen = reinterpret_cast<int32_t*>(word + E);  // WHOLE: [32][top], then 2 E + 32 integers
+    int32_t* chosen = reinterpret_cast<int32_t*>(word + E);  // WHOLE: [kWholeTokens][top], then 2 E + 32 integers
     for (int e = threadIdx.x; e < E; e += blockDim.x) word[e] = 0;
     float b[P], bias_most = 0.0f;
 #pragma unroll
@@ -444,7 +446,7 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
     }
     cluster_arrive();
     cluster_wait();
-    int32_t *at = chosen + kTokens * a.top, *before = at + E;
+    int32_t *at = chosen + kWholeTokens * a.top, *before = at + E;
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int all = 0, ahead = 0;
 #pragma unroll
@@ -576,7 +578,7 @@ template <typename T, int P, bool WHOLE>
 int launch_select(const spk_route_scores_args& a, uint32_t* words, int n_words, cudaStream_t s) {
     const int tokens = tokens_of(a.n);
     // 64-bit scores of a warp are kept in shared memory: as many warps as fit
-    const int per = 16 * a.experts, extra = 4 * a.experts + (WHOLE ? 4 * (kTokens * a.top + 2 * a.experts + 32) : 0);
+    const int per = 16 * a.experts, extra = 4 * a.experts + (WHOLE ? 4 * (kWholeTokens * a.top + 2 * a.experts + 32) : 0);
     int warps = !WHOLE ? min(tokens, 16) : tokens < 8 ? 8 : tokens;  // eight at least hand out the rows
     while (warps * per + extra > 200 * 1024) warps /= 2;
     const int bytes = warps * per + extra;

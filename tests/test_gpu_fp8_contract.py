@@ -241,3 +241,13 @@ def test_products_of_scales_beyond_32_bits(dev, n, k, f):
     check_linear(k8.linear_fp8(x, sx, w, sw, out_dtype=F32), x, sx, w, sw)
     sx[0], sw[:, 0] = 0.0, 2.0 ** 120
     check_linear(k8.linear_fp8(x, sx, w, sw, out_dtype=F32), x, sx, w, sw)
+
+
+@pytest.mark.parametrize("n", [7, 8, 9, 63, 64, 113, 120, 127, 128])
+@pytest.mark.parametrize("experts,top", [(16, 16), (256, 32), (1000, 32)])
+def test_routes_that_one_cluster_hands_out(dev, n, experts, top):
+    """One to sixteen tokens a CTA and up to 32 choices each: the most that a launch of one cluster keeps."""
+    logits = torch.randn(n, experts, generator=gen(n + top))
+    r = kr.route_by_scores(logits.to(dev), top)
+    check_route(r, logits, top)
+    rows_in_order(r, experts)
