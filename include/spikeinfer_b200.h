@@ -783,6 +783,8 @@ typedef struct spk_linear_fp8_args {
     uint32_t* status;
 } spk_linear_fp8_args;
 int spk_linear_fp8(const spk_linear_fp8_args* args, void* stream);
+/* The form that spk_linear_fp8 takes for these sizes: 16 times the rows of a tile (16, 32, 64, 128, or 256 by a pair of CTAs), plus the parts that k is cut into; 0 where a size is below 1. */
+int spk_linear_fp8_form(int64_t n, int64_t k, int64_t features);
 
 /* Experts chosen by scores.  Per token: s = softmax(logits) or 1 / (1 + exp(-logits)), c = s + bias (bias may be NULL).  groups > 1: the experts are cut into
  * `groups` equal runs, a group counts the sum of its best two c, and only the best top_groups groups stay.  ids [n, top] <- the best c in falling order,

@@ -326,6 +326,7 @@ SIGNATURES = {
     "spk_rms_residual_fp8": (c_int, [POINTER(RmsResidualFp8Args), c_void_p]),
     "spk_quantize_fp8": (c_int, [POINTER(QuantizeFp8Args), c_void_p]),
     "spk_linear_fp8": (c_int, [POINTER(LinearFp8Args), c_void_p]),
+    "spk_linear_fp8_form": (c_int, [c_int64] * 3),
     "spk_route_scores_workspace_bytes": (c_int64, [c_int64, c_int]),
     "spk_route_scores": (c_int, [POINTER(RouteScoresArgs), c_void_p]),
     "spk_gelu_tanh": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),

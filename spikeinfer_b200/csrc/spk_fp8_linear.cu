@@ -758,19 +758,42 @@ int launch_tiles(const spk_linear_fp8_args& a, cudaStream_t s) {
     return SPK_OK;
 }
 
-// Parts of k: as many as leave the clusters on the chip at once (148 SMs in groups of 16 to 18 hold 64 or more of two CTAs, 32 of four, 16 of eight).  One / two / four parts, us: 16 x 3584 x
-// 4608 11.5 / 8.7 / 12.4 (36 clusters of four: two waves), 64 x 18944 x 3584 51.8 / 28.0 / 18.8, 64 x 4864 x 896 17.7 / 11.5 / 8.8 (eight 8.0),
-// 16 x 18944 x 1024 in four / eight 13.7 / 9.7, 64 x 18944 x 2048 17.7 / 23.9, 1 x 896 x 4864 5.5 / 5.4 / 8.3 whole / in two / four.
+// The form of a product: rows of a tile (16, 32, 64: fp8_rows_kernel; 128; 256: by pairs) and parts of k.
+struct Form {
+    int rows, parts;
+};
+Form form_of(int64_t n, int64_t k, int64_t features) {
+    const int64_t blocks = (k + kBlock - 1) / kBlock, fblocks = (features + 127) / 128;
+    if (n <= 64) {
+        // Parts of k: as many as leave the clusters on the chip at once (148 SMs in groups of 16 to 18 hold 64 or more of two CTAs, 32 of four, 16 of eight).  One / two / four parts, us: 16 x 3584 x
+        // 4608 11.5 / 8.7 / 12.4 (36 clusters of four: two waves), 64 x 18944 x 3584 51.8 / 28.0 / 18.8, 64 x 4864 x 896 17.7 / 11.5 / 8.8 (eight 8.0),
+        // 16 x 18944 x 1024 in four / eight 13.7 / 9.7, 64 x 18944 x 2048 17.7 / 23.9, 1 x 896 x 4864 5.5 / 5.4 / 8.3 whole / in two / four.
+        const int parts = fblocks <= 8 && blocks >= 16 ? 8 : fblocks <= 32 && blocks >= 8 ? 4 : fblocks <= 64 && blocks >= 4 ? 2 : 1;
+        return {n <= 16 ? 16 : n <= 32 ? 32 : 64, parts};
+    }
+    // Tiles of 128 x 128, or of 256 x 256 by pairs of CTAs, which take 1.6 times as long a wave (8192 x 3584 x 18944: 733 / 612 us; 1171 x 896 x 4864, three waves of 380 tiles against
+    // two of 95: 14.3 / 16.4).  Few tiles: parts of k as above (1171 x 4864 x 896, 70 tiles: 19.2 us whole, 14.9 in two).
+    const int64_t tiles = (n + 127) / 128 * fblocks, pairs = (n + 255) / 256 * ((features + 255) / 256);
+    if (tiles <= 32 && blocks >= 16) return {128, 4};
+    if (tiles <= 72 && blocks >= 8) return {128, 2};
+    return {8 * ((pairs + 73) / 74) < 5 * ((tiles + 147) / 148) ? 256 : 128, 1};
+}
+
 template <int TN>
-int dispatch(const spk_linear_fp8_args& a, cudaStream_t s) {
-    const int64_t ctas = (a.features + 127) / 128, blocks = (a.k + kBlock - 1) / kBlock;
-    if (ctas <= 8 && blocks >= 16) return launch_rows<TN, 8>(a, s);
-    if (ctas <= 32 && blocks >= 8) return launch_rows<TN, 4>(a, s);
-    if (ctas <= 64 && blocks >= 4) return launch_rows<TN, 2>(a, s);
+int launch_parts(const spk_linear_fp8_args& a, int parts, cudaStream_t s) {
+    if (parts == 8) return launch_rows<TN, 8>(a, s);
+    if (parts == 4) return launch_rows<TN, 4>(a, s);
+    if (parts == 2) return launch_rows<TN, 2>(a, s);
     return launch_rows<TN, 1>(a, s);
 }
 
 }  // namespace
+
+extern "C" int spk_linear_fp8_form(int64_t n, int64_t k, int64_t features) {
+    if (n < 1 || k < 1 || features < 1) return 0;
+    const Form f = form_of(n, k, features);
+    return f.rows * 16 + f.parts;
+}
 
 extern "C" int spk_linear_fp8(const spk_linear_fp8_args* args, void* stream) {
     SpkRange nvtx_range("spk_linear_fp8");
@@ -786,14 +809,12 @@ extern "C" int spk_linear_fp8(const spk_linear_fp8_args* args, void* stream) {
     if (a.n > 0x7fffff00LL || a.features > 0x7fffff00LL || a.k > 0x7fffff00LL || a.x_stride >= 1LL << 40 || a.w_stride >= 1LL << 40) return SPK_ERR_TOO_LARGE;
     if (a.x == nullptr || a.w == nullptr || a.x_scales == nullptr || a.w_scales == nullptr || a.out == nullptr) return SPK_ERR_NULL_POINTER;
     cudaStream_t s = spk_stream(stream);
-    if (a.n <= 16) return dispatch<16>(a, s);
-    if (a.n <= 32) return dispatch<32>(a, s);
-    if (a.n <= 64) return dispatch<64>(a, s);
-    // Tiles of 128 x 128, or of 256 x 256 by pairs of CTAs, which take 1.6 times as long a wave (8192 x 3584 x 18944: 733 / 612 us; 1171 x 896 x 4864, three waves of 380 tiles against
-    // two of 95: 14.3 / 16.4).  Few tiles: parts of k as above (1171 x 4864 x 896, 70 tiles: 19.2 us whole, 14.9 in two).
-    const int64_t tiles = (a.n + 127) / 128 * ((a.features + 127) / 128), pairs = (a.n + 255) / 256 * ((a.features + 255) / 256);
-    if (tiles <= 32 && blocks >= 16) return launch_tiles<128, 1, 4>(a, s);
-    if (tiles <= 72 && blocks >= 8) return launch_tiles<128, 1, 2>(a, s);
-    if (8 * ((pairs + 73) / 74) < 5 * ((tiles + 147) / 148)) return launch_tiles<256, 2, 1>(a, s);
+    const Form f = form_of(a.n, a.k, a.features);
+    if (f.rows == 16) return launch_parts<16>(a, f.parts, s);
+    if (f.rows == 32) return launch_parts<32>(a, f.parts, s);
+    if (f.rows == 64) return launch_parts<64>(a, f.parts, s);
+    if (f.parts == 4) return launch_tiles<128, 1, 4>(a, s);
+    if (f.parts == 2) return launch_tiles<128, 1, 2>(a, s);
+    if (f.rows == 256) return launch_tiles<256, 2, 1>(a, s);
     return launch_tiles<128, 1, 1>(a, s);
 }

@@ -5,6 +5,8 @@ import torch
 
 from spikeinfer_b200.kernels import fp8 as k8
 
+from test_gpu_fp8_contract import FORMS
+
 
 def test_workspace_of_many_tokens_holds_counts_by_chunks(lib):
     """A bit for every token and expert, 32 to a word, four words at a time; beyond 1024 words a count for every 64 of them, and the sums."""
@@ -38,3 +40,16 @@ def test_weights_that_are_not_finite_stay_alone():
         rest[:128, 256:] = rest[128:, :128] = rest[128:, 256:] = False
         assert torch.equal(values[rest], want.float()[rest])
         assert (values[128:, :128] == 0).sum() >= 72 * 128 - 1  # next to 3e38 there is nothing left of the others
+
+
+def test_every_form_of_the_product_is_tested_beyond_its_rings(lib):
+    """The sizes of test_products_of_every_form take the forms that they stand for, all that a sweep of sizes meets, and long parts of k; a changed rule shows here."""
+    form = lambda n, k, f: divmod(lib.spk_linear_fp8_form(n, k, f), 16)
+    for want, sizes in FORMS.items():
+        assert all(form(*size) == want for size in sizes), (want, sizes)
+        assert max(-(-k // 128) // want[1] for _, k, _ in sizes) >= 33
+    met = {form(n, k, f) for n in (1, 20, 40, 65, 130, 600, 1171, 8192) for k in (100, 900, 2100, 4864, 18_944) for f in (100, 900, 2000, 4864, 8192, 18_944)}
+    assert met == set(FORMS)
+    assert lib.spk_linear_fp8_form(0, 5, 5) == lib.spk_linear_fp8_form(5, 0, 5) == lib.spk_linear_fp8_form(5, 5, 0) == 0
+    # tiles of 128 x 128: more than one a CTA (148 SMs), and more blocks of k than the ring of scales holds (four groups of eight)
+    assert any(-(-n // 128) * -(-f // 128) > 148 and k > 32 * 128 for n, k, f in FORMS[128, 1])

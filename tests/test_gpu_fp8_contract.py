@@ -5,10 +5,11 @@ import pytest
 import torch
 
 from oracle import fp8_oracle as fo
+from spikeinfer_b200 import _lib
 from spikeinfer_b200.kernels import fp8 as k8
 from spikeinfer_b200.kernels import routing as kr
 
-from test_gpu_fp8_ops import BF, F32, FP8, check_linear, check_route, gen, operands
+from test_gpu_fp8_ops import BF, F32, FP8, HALF, NORM, U, check_linear, check_route, gen, operands
 
 pytestmark = pytest.mark.gpu
 
@@ -251,3 +252,65 @@ def test_routes_that_one_cluster_hands_out(dev, n, experts, top):
     r = kr.route_by_scores(logits.to(dev), top)
     check_route(r, logits, top)
     rows_in_order(r, experts)
+
+
+# ---- every form, beyond the first turn of its rings --------------------------------------------------------------------
+# (rows of a tile, parts of k) of the sizes that take it; every CTA has 33 or more blocks of 128 columns, so that stages, accumulators and groups of scales are used again
+FORMS = {(rows, parts): [(n, 4300 * parts, f)] for rows, n in ((16, 13), (32, 29), (64, 61)) for parts, f in ((1, 8200), (2, 4120), (4, 1100), (8, 300))}
+FORMS |= {(128, 4): [(130, 17_100, 200)], (128, 2): [(300, 8500, 1500)], (128, 1): [(1171, 4300, 1200), (1171, 4300, 4864), (1171, 896, 4864)],  # one tile a CTA, two and three
+          (256, 1): [(2600, 4300, 4000), (2600, 3584, 4000)]}
+
+
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+@pytest.mark.parametrize("rows,parts,n,k,f", [(*form, *size) for form, sizes in FORMS.items() for size in sizes])
+def test_products_of_every_form(dev, rows, parts, n, k, f, out_dtype):
+    assert _lib.load().spk_linear_fp8_form(n, k, f) == 16 * rows + parts
+    x, sx, w, sw = operands(n, k, f, dev, n + k + f)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = k8.linear_fp8(x, sx, w, sw, out_dtype=out_dtype, status=status)
+    want, size = fo.linear(x, sx, w, sw)
+    tol = (132 * 2.0 ** -23 + (3 + -(-k // 128)) * U) * size  # as check_linear
+    assert ((out.double() - want).abs() <= tol + HALF[out_dtype] * (want.abs() + tol)).all()
+    assert torch.equal(out, k8.linear_fp8(x, sx, w, sw, out_dtype=out_dtype)) and int(status.item()) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu_gate"])
+@pytest.mark.parametrize("n,width", [(600, 4864), (600, 3502), (600, 3501), (8192, 4864)])
+def test_activations_of_several_blocks_at_a_time(dev, n, width, act, dtype):
+    """Two blocks at a time from 16384 on, four (16-bit rows on 16-byte boundaries) from 262144 on; bounds as test_quantize counts them."""
+    g = torch.Generator(device=dev).manual_seed(n + width)
+    z = (3 * torch.randn(n, width * (2 if act == "silu_gate" else 1), generator=g, device=dev)).to(dtype)
+    q, scales = k8.quantize_fp8(z, act)
+    v, rel = fo.activation(z, act), (1300 if act == "gelu_tanh" else 64) * U
+    blocks = -(-width // 128)
+    most = torch.nn.functional.pad(v.abs(), (0, blocks * 128 - width)).view(n, blocks, 128).amax(2).clamp(min=fo.LEAST)
+    assert ((scales.t().double() - most / 448).abs() <= (rel + 2 * U) * most / 448).all()
+    s = scales.double().t().repeat_interleave(128, 1)[:, :width]
+    off = (q.double() * s - v).abs()
+    keep = v.abs() > 1e-4 * 448 * s
+    assert (off <= 0.5 * fo.e4m3_step(v / s) * s * (1 + 64 * U) + (rel + 4 * U) * v.abs())[keep].all()
+    assert (off <= 1.01 * 2.0 ** -9 * s)[~keep].all()
+    few = k8.quantize_fp8(z[-5:].contiguous(), act)  # a block's values do not depend on how many are taken at once
+    assert torch.equal(q[-5:].float(), few[0].float()) and torch.equal(scales[:, -5:], few[1])
+
+
+@pytest.mark.parametrize("stream,delta_dtype", [(BF, BF), (BF, None), (F32, F32), (F32, BF), (F32, None)])
+@pytest.mark.parametrize("n,width", [(8192, 3584), (5001, 896), (9000, 128), (4000, 8192), (4000, 1000)])
+def test_boundaries_of_many_rows_a_cta(dev, n, width, stream, delta_dtype):
+    """The streaming form gives a CTA more rows than it has stages (three): up to 19 here."""
+    g = torch.Generator(device=dev).manual_seed(n + width)
+    x = torch.randn(n, width, generator=g, device=dev).to(stream)
+    delta = None if delta_dtype is None else torch.randn(n, width, generator=g, device=dev).to(delta_dtype)
+    w, eps = 1 + 0.3 * torch.randn(width, generator=g, device=dev), 1e-5
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    x_out, out = x.clone(), torch.empty(n, width, device=dev)
+    q, scales = k8.rms_residual_fp8(x_out, w, eps=eps, delta=delta, x_out=x_out, out=out, status=status)  # in place
+    y = x.float() if delta is None else x.float() + delta.float()
+    assert torch.equal(x_out, y.to(stream))  # one rounding to 32 bits, and to the stream's
+    v = fo.rms_norm(x_out, w, eps)
+    assert ((out.double() - v).abs() <= (NORM + U) * (1 + 2 * U) * v.abs()).all()
+    is_quotient(q, scales, out)
+    short = torch.empty(n, width, dtype=BF, device=dev)
+    q2, s2 = k8.rms_residual_fp8(x, w, eps=eps, delta=delta, out=short, status=status)
+    assert torch.equal(short, out.to(BF)) and torch.equal(q2.float(), q.float()) and torch.equal(s2, scales) and int(status.item()) == 0
