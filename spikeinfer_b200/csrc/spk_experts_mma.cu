@@ -201,8 +201,7 @@ experts_kernel(const spk_experts_args a, const int blocks, const int ktiles) {
         }
     }
     if (S > 1) {
-        cluster_arrive();
-        cluster_wait();
+        cluster_sync();
         if (warp >= 2) {  // every CTA adds and writes its own tokens
             constexpr int J = 32 / S;
             const int quad = warp & 3, j0 = part * J, n = min(J, rows - j0);
@@ -224,8 +223,7 @@ experts_kernel(const spk_experts_args a, const int blocks, const int ktiles) {
                 else store_plain<J>(a, row0 + j0, n, f, x, y);
             }
         }
-        cluster_arrive();
-        cluster_wait();  // no CTA leaves while its sums are being read
+        cluster_sync();  // no CTA leaves while its sums are being read
     }
     __syncwarp();
     tc_fence_before();

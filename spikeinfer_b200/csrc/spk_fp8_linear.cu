@@ -291,8 +291,7 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
         }
     }
     if (S > 1) {
-        cluster_arrive();
-        cluster_wait();
+        cluster_sync();
         if (warp >= 4) {  // every CTA adds and writes its own tokens
             constexpr int J = TN / S / (Sh::kWriters / 4);
             const int quad = warp & 3, j0 = part * (TN / S) + (warp - 4) / 4 * J;
@@ -311,8 +310,7 @@ fp8_rows_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_cons
                 if (j0 + j < a.n && f < a.features) put(a, j0 + j, f, y);
             }
         }
-        cluster_arrive();
-        cluster_wait();  // no CTA leaves while its sums are being read
+        cluster_sync();  // no CTA leaves while its sums are being read
     }
     __syncwarp();
     tc_fence_before();
@@ -487,8 +485,7 @@ fp8_tiles_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_con
     tc_fence_before();
     __syncthreads();
     if (CG == 2) {  // the pair's barriers are set up
-        cluster_arrive();
-        cluster_wait();
+        cluster_sync();
     }
     tc_fence_after();
     const uint32_t tmem = bars->tmem;
@@ -631,8 +628,7 @@ fp8_tiles_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_con
         }
     }
     if (S > 1) {
-        cluster_arrive();
-        cluster_wait();
+        cluster_sync();
         if (warp >= 4) {  // every CTA adds and writes its own columns, two warps those of a token
             constexpr int J = NF / S / (kWriters / 4);
             const int r = (warp & 3) * 32 + lane, j0 = part * (NF / S) + (warp - 4) / 4 * J;
@@ -647,10 +643,8 @@ fp8_tiles_kernel(const __grid_constant__ spk_linear_fp8_args a, const __grid_con
             if (t < a.n) put_row<J>(a, vec, t, f, v);
         }
     }
-    __syncwarp();
     if (S > 1 || CG == 2) {
-        cluster_arrive();
-        cluster_wait();  // no CTA leaves while its sums are being read, or its partner works in its memory
+        cluster_sync();  // no CTA leaves while its sums are being read, or its partner works in its memory
     }
     // Behind the pair's barrier the even CTA has seen its last commit, so its arrivals here are all but made, however long the product took (a wait's limit is meant for one phase).
     if (CG == 2 && rank != 0 && warp == 1 && !mbar_wait(smem_u32(&bars->done), 0)) *abort = 1;

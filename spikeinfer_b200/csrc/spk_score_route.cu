@@ -444,8 +444,7 @@ score_select_kernel(const __grid_constant__ spk_route_scores_args a, uint32_t* w
             for (int k = 0; k <= behind; ++k) words[static_cast<int64_t>(e) * row + blockIdx.x + k] = k == 0 ? word[e] : 0u;
         return;
     }
-    cluster_arrive();
-    cluster_wait();
+    cluster_sync();
     int32_t *at = chosen + kWholeTokens * a.top, *before = at + E;
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int all = 0, ahead = 0;

@@ -55,7 +55,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 // Barrier of a cluster's CTAs.  Instructions with .aligned want the whole warp at once, which code before them (one lane's work, a loop that ends earlier for some lanes) does not
-// promise: so here, and for the tensor memory below.
+// promise: so here, and for the tensor memory below.  (Arrival and wait with a convergence each, or one more in front of both: 8192 x 3584 x 18944 in 8 bits 585 us, with one 568.)
 __device__ __forceinline__ void cluster_arrive() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -63,6 +63,10 @@ __device__ __forceinline__ void cluster_arrive() {
 __device__ __forceinline__ void cluster_wait() {
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
