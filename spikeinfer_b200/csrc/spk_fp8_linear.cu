@@ -6,13 +6,15 @@
 // fp8_rows_kernel (up to 64 rows): CTA = (128 features, all rows, part of k).  The weights are the M operand, the tokens the N operand: a few decoded tokens cost a
 // narrow MMA and every lane of the accumulators is a feature.  Where few CTAs would stream the weights, a cluster of S shares the blocks of k; the parts meet in shared
 // memory and are added in the order of the CTAs.  64 x 3584 x 18944: 17.6 us, 3.8 TB/s of weights (0.61 of the copy rate; set-up and drain are 4 us of it).
-// fp8_tiles_kernel (more rows): the tokens are the M operand, below.  8192 x 3584 x 18944: 574 us, 1.94 PFLOP/s (1.16 of the library's measured bf16 rate).
+// fp8_tiles_kernel (more rows): the tokens are the M operand, below.  8192 x 3584 x 18944: 564 us, 1.97 PFLOP/s (1.18 of the library's measured bf16 rate; up to 600 where the GPU has been at its power
+// limit before).
 //
-// What bounds the large products: the hand-over of accumulators.  A block of 128 x 256 is 512 cycles of MMAs; its sums are read, scaled and added in some 500 cycles by
-// eight warps, and with two accumulators the way from the last MMA through the writers to the next MMA into the same columns counts (about 1150 cycles a block).
+// What bounds the large products: two lanes of work of nearly the same length.  With parts taken out in turn, the MMAs alone (copies, barriers) were 480 us, everything but the MMAs (sums read from
+// tensor memory, scaled, added, stored) 455, both 570.  480 is half the nominal e4m3 rate; why is not known.  A block of 128 x 256 is 512 cycles of MMAs at the nominal rate, its sums are read, scaled
+// and added in some 500 cycles by eight warps, and with two accumulators the way from the last MMA through the writers to the next MMA into the same columns counts as well (some 1150 cycles a block).
 // Scales that are powers of two for 32 columns could stay in the MMA; these are 32-bit and for 128.
-// Measured on the way, us for 8192 x 3584 x 18944: one accumulating warpgroup per feature block 1680; products of pairs (fma.rn.f32x2) 656, one by one 606; barriers for every
-// block's scales 703, for eight blocks 600; an arrival with cluster scope on the pair's barrier 1240, without 640; 16 writing warps 606, eight 600.
+// Steps on the way, us before / after for 8192 x 3584 x 18944: one accumulating warpgroup per feature block 1680; barriers for every block's scales / for eight blocks 703 / 600; products of pairs
+// (fma.rn.f32x2) / one by one 656 / 606; an arrival with cluster scope on the pair's barrier / without 1240 / 640; 16 writing warps / eight 606 / 600.
 #include <cuda.h>
 #include <cuda_fp8.h>
 #include <float.h>
@@ -765,8 +767,8 @@ Form form_of(int64_t n, int64_t k, int64_t features) {
         const int parts = fblocks <= 8 && blocks >= 16 ? 8 : fblocks <= 32 && blocks >= 8 ? 4 : fblocks <= 64 && blocks >= 4 ? 2 : 1;
         return {n <= 16 ? 16 : n <= 32 ? 32 : 64, parts};
     }
-    // Tiles of 128 x 128, or of 256 x 256 by pairs of CTAs, which take 1.6 times as long a wave (8192 x 3584 x 18944: 733 / 612 us; 1171 x 896 x 4864, three waves of 380 tiles against
-    // two of 95: 14.3 / 16.4).  Few tiles: parts of k as above (1171 x 4864 x 896, 70 tiles: 19.2 us whole, 14.9 in two).
+    // Tiles of 128 x 128, or of 256 x 256 by pairs of CTAs, which take 1.6 times as long a wave (8192 x 3584 x 18944: 720 / 564 us; 1171 x 896 x 4864, three waves of 380 tiles against
+    // two of 95: 14.9 / 16.8).  Few tiles: parts of k as above (1171 x 4864 x 896, 70 tiles: 19.2 us whole, 14.9 in two).
     const int64_t tiles = (n + 127) / 128 * fblocks, pairs = (n + 255) / 256 * ((features + 255) / 256);
     if (tiles <= 32 && blocks >= 16) return {128, 4};
     if (tiles <= 72 && blocks >= 8) return {128, 2};

@@ -6,8 +6,8 @@
 // A block of 128 columns is the four-column groups of one warp, so its largest magnitude is one warp reduction away.  scale = most / 448 (448: the
 // largest e4m3 value), value = round(v / scale), saturating: NaN stays NaN and is no candidate for the largest, an infinity counts as the
 // largest finite value.  A block below 2^-100 is scaled as if its largest magnitude was that, so that no reciprocal overflows.
-// Both quotients are what a 32-bit division gives, by Markstein's correction of a product with the reciprocal (q + (a - q b) / b, the remainder without a rounding), two values an instruction (8192 x 3584 boundary 38.9 -> 39.9 us, gate of
-// 8192 x 18944 131 -> 125, no activation 78 -> 84, gelu of 8192 x 4864 33.4 -> 34.8; one value an instruction 40.9, 128, 86, 35.5).
+// Both quotients are what a 32-bit division gives, by Markstein's correction of a product with the reciprocal (q + (a - q b) / b, the remainder without a rounding), two values an instruction.  Products
+// alone / corrected / one value an instruction, us: 8192 x 3584 boundary 38.9 / 39.9 / 40.9, gate of 8192 x 18944 131 / 125 / 128, no activation 78 / 84 / 86, gelu of 8192 x 4864 33.4 / 34.8 / 35.5.
 // 16-bit values over a scale of few bits lie exactly between two e4m3 values once in a thousand, where the product alone, or a scale that is off by a unit, takes the other one.
 #include <cuda_fp8.h>
 #include <float.h>
@@ -170,7 +170,8 @@ __device__ __forceinline__ void put8(void* q, int64_t q_stride, float* scales, i
     if (c % 128 == 0) scales[(c >> 7) * scale_stride + t] = scale;
 }
 
-// One CTA per row, C columns a thread and group.  Everything that does not depend on the row's sum is asked for at once.
+// One CTA per row, C columns a thread and group.  Everything that does not depend on the row's sum is asked for at once.  (V = 8, rows of more than 8192 fp32 or 16384 bf16 columns, keeps the row in the
+// registers of up to 1024 threads: 32 or 64 of them, so that 0.5 to 2.6 KB a thread go through local memory.)
 template <typename TX, typename TD, int V, int VEC, int MOST>
 __global__ void __launch_bounds__(MOST)
 boundary8_kernel(const spk_rms_residual_fp8_args p) {
@@ -349,8 +350,8 @@ int launch_stream(const spk_rms_residual_fp8_args& p, int stage, cudaStream_t s)
     return SPK_OK;
 }
 
-// Whether a batch goes to the streaming form, and its launch: no expert rows, enough rows, and 16-bit or narrow ones (8192 rows, the form above / streaming, us: 3584 bf16 106 / 37, 896 bf16
-// 17.0 / 11.8, 896 fp32 22.9 / 20.5, 3584 fp32 61 / 72).  Narrow rows have two warps each (one 14.3 and 27.1, four 14.4 and 23.4).
+// Whether a batch goes to the streaming form, and its launch: no expert rows, enough rows, and 16-bit or narrow ones (8192 rows, the form above / streaming, us: 3584 bf16 104 / 38, 896 bf16
+// 16.7 / 12.3, 896 fp32 19.9 / 17.2; 3584 fp32 61 / 72).  Narrow rows have two warps each (one 14.3 and 27.1, four 14.4 and 23.4).
 template <typename TX, typename TD>
 bool stream_boundary8(const spk_rms_residual_fp8_args& p, cudaStream_t s, int* rc) {
     constexpr int F = sizeof(TX) / 2;
@@ -429,8 +430,7 @@ int launch_quantize8(const spk_quantize_fp8_args& p, cudaStream_t s) {
     auto at = [&](int e) { return p.width % e == 0 && p.z_stride % e == 0 && reinterpret_cast<uintptr_t>(p.z) % (e * sizeof(T)) == 0; };
     constexpr int e = 16 / sizeof(T);
     const bool wide = at(e);
-    // One / two / four blocks at a time, us: 37 x 4864 bf16 gelu 1.85 / 2.11 / 2.96, 512 rows 4.6 / 4.3 / 5.1, 8192 rows 40.4 / 36.4 / 35.3; 8192 x 18944 gate 149 / 132 / 127 (with 256 threads a CTA), without activation
-    // 103 / 89 / 92.
+    // One / two / four blocks at a time, us: 37 x 4864 bf16 gelu 1.64 / 1.75 / 2.47, 512 rows 4.1 / 3.7 / 4.6, 8192 rows 39.0 / 34.1 / 33.9; 8192 x 18944 gate 141 / 128 / 122, without activation 100 / 82 / 87.
     constexpr int U4 = ACT != SPK_ACT_NONE && sizeof(T) == 2 ? 4 : 2;
     const int u = blocks < 16384 ? 1 : wide && blocks >= 262144 ? U4 : 2, per = kQuantThreads / (wide ? 128 / e : 32) * u;
     const unsigned grid = static_cast<unsigned>((blocks + per - 1) / per);

@@ -5,7 +5,8 @@
 // the best one dropped) is beyond what the scores can be off by, it has the sign of the exact one.  Where one is not, the groups, or the experts that can be among the chosen, are
 // compared in 64 bits.  (64 bits for every token: 8191 rows of 256 experts in eight groups 94 us, 64 rows 44; for the whole of a token that is not settled: 49 and 13; so, with the layout's loads side by side, 34 and 9.5.)
 //
-// What bounds it: some 1300 instructions a token (scores 200, groups 250, choices 500, weights 100) and their latency; reading the logits would take 1.4 of the 34 us.
+// What bounds it: some 1300 instructions a token (scores 200, groups 250, choices 500, weights 100) and their latency; reading the logits would take 1.4 of the 35 us.  The form of more than 128 tokens
+// has 64 registers (two CTAs of 512 threads on an SM) and spills 64 to 100 bytes a thread up to 256 experts, 0.2 KB up to 512, 0.9 KB beyond.
 //
 // A CTA's 32 tokens leave one word per expert, a bit for every token that chose it (a token chooses an expert once).  A pair's row is what the words ahead count, and the
 // bits below its own: no order of arrival enters, so the rows are the same every time.  Up to 128 tokens: a cluster's CTAs read one another's words, one launch.
