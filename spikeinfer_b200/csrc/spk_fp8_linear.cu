@@ -5,7 +5,7 @@
 //
 // fp8_rows_kernel (up to 64 rows): CTA = (128 features, all rows, part of k).  The weights are the M operand, the tokens the N operand: a few decoded tokens cost a
 // narrow MMA and every lane of the accumulators is a feature.  Where few CTAs would stream the weights, a cluster of S shares the blocks of k; the parts meet in shared
-// memory and are added in the order of the CTAs.  64 x 3584 x 18944: 17.6 us, 3.8 TB/s of weights (0.61 of the copy rate; set-up and drain are 4 us of it).
+// memory and are added in the order of the CTAs.  64 x 3584 x 18944: 17.7 us, 3.8 TB/s of weights (0.61 of the copy rate; set-up and drain are 4 us of it).
 // fp8_tiles_kernel (more rows): the tokens are the M operand, below.  8192 x 3584 x 18944: 564 us, 1.97 PFLOP/s (1.18 of the library's measured bf16 rate; up to 600 where the GPU has been at its power
 // limit before).
 //
@@ -768,7 +768,7 @@ Form form_of(int64_t n, int64_t k, int64_t features) {
         return {n <= 16 ? 16 : n <= 32 ? 32 : 64, parts};
     }
     // Tiles of 128 x 128, or of 256 x 256 by pairs of CTAs, which take 1.6 times as long a wave (8192 x 3584 x 18944: 720 / 564 us; 1171 x 896 x 4864, three waves of 380 tiles against
-    // two of 95: 14.9 / 16.8).  Few tiles: parts of k as above (1171 x 4864 x 896, 70 tiles: 19.2 us whole, 14.9 in two).
+    // two of 95: 14.9 / 16.8).  Few tiles: parts of k as above (1171 x 4864 x 896, 70 tiles: 19.2 us whole, 15.0 in two).
     const int64_t tiles = (n + 127) / 128 * fblocks, pairs = (n + 255) / 256 * ((features + 255) / 256);
     if (tiles <= 32 && blocks >= 16) return {128, 4};
     if (tiles <= 72 && blocks >= 8) return {128, 2};
