@@ -97,7 +97,7 @@ __device__ __forceinline__ void put(const spk_linear_fp8_args& a, int64_t t, int
 }
 
 // A block's sum is multiplied by the product of its scales.  Where that is beyond the 32-bit numbers while both scales are not (1e20 times 1e20, beside a sum of zero too), what a thread has
-// added up is put aside, and its outputs are summed up here from the operands, some hundred times as slow: a sum times the smaller scale, times the larger one, so that nothing on the way
+// added up is put aside, and its outputs are summed up here from the operands, up to 500 times as slow: a sum times the smaller scale, times the larger one, so that nothing on the way
 // overflows unless the term does.  (A branch for every block in the loops that read tensor memory took 2 to 12 % of all products.)  A product below the normal numbers is taken as it is, to
 // within 2^-150: scales of 2^-100 / 448, those of blocks of zeros, are met beside small ones.
 __device__ __forceinline__ bool is_far(float x, float w) { return fabsf(x * w) == INFINITY && fabsf(x) <= FLT_MAX && fabsf(w) <= FLT_MAX; }
